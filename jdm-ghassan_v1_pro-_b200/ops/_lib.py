@@ -108,6 +108,7 @@ STATUS_NAMES = {
     301: "bad argument detected on device",
     401: "decode step: a wait for the other CTAs ran out",
     402: "decode step: a bulk copy of weight rows never signalled its barrier",
+    303: "paged cache: a key or value was not finite; it is held as zero",
     302: "expert parallelism: more rows were routed to this rank's experts than its buffers hold (raise b200.ep_capacity)",
 }
 
