@@ -1,5 +1,8 @@
 // Attention over the paged 8-bit cache (interface in gb_paged.h): one warp per query head, keys page by page.
-#include "paged_util.cuh"
+#include <algorithm>
+#include <atomic>
+
+#include "paged_attn.cuh"
 
 namespace gb {
 
@@ -54,25 +57,80 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const __grid_constant__
   }
 }
 
+int pg_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { (void)cudaGetLastError(); return 148; }
+  if ((n = known[dev].load(std::memory_order_relaxed))) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { (void)cudaGetLastError(); return 148; }
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 }  // namespace gb
 
 using namespace gb;
 
-extern "C" int gb_paged_attn(const gb_paged* a, const void* q, long long ld_q, int H, float scale, int window, void* out, long long ld_o,
-                             cudaStream_t st) {
+// The sequences from b0 on, at most PG_MOST_SEQS of them.
+static PgAttn gb_paged_some(const PgAttn& p, int b0) {
+  PgAttn s = p;
+  s.a.B = std::min(PG_MOST_SEQS, p.a.B - b0);
+  s.a.table += (long long)b0 * p.a.W;
+  s.a.start += b0;
+  if (s.a.count) {
+    s.a.first += b0;
+    s.a.count += b0;
+  } else {                                                 // rows are counted from a launch's first sequence
+    s.q = (const char*)p.q + 2ll * b0 * p.ld_q;
+    s.out = (char*)p.out + 2ll * b0 * p.ld_o;
+    s.a.rows = std::max(0ll, p.a.rows - b0);
+  }
+  return s;
+}
+
+static int gb_paged_attn_args(const gb_paged* a, int H, int window) {
   if (const int rc = gb_paged_check(a)) return rc;
+  if (H <= 0 || H % a->KV || window < 0 || H > 65535) return -1;
+  if ((long long)std::min(a->B, PG_MOST_SEQS) * a->W * a->KV > 0x7fffffffll) return -3;
+  return 0;
+}
+
+extern "C" long long gb_paged_attn_ws(const gb_paged* a, int H, int window) {
+  if (const int rc = gb_paged_attn_args(a, H, window)) return rc;
   if (a->B == 0 || a->max_new == 0 || a->rows == 0) return 0;
-  if (H <= 0 || H % a->KV || !(scale > 0.f) || window < 0) return -1;
+  PgAttn p = {*a, nullptr, 0, H, 0.f, window, nullptr, 0, nullptr};
+  if ((long long)a->max_new * (H / a->KV) <= PG_TOKEN_ROWS) return pg_token_ws(gb_paged_some(p, 0));
+  return 0;
+}
+
+extern "C" int gb_paged_attn(const gb_paged* a, const void* q, long long ld_q, int H, float scale, int window, void* out, long long ld_o,
+                             float* ws, long long ws_floats, cudaStream_t st) {
+  if (const int rc = gb_paged_attn_args(a, H, window)) return rc;
+  if (!(scale > 0.f)) return -1;
+  if (a->B == 0 || a->max_new == 0 || a->rows == 0) return 0;
   const long long width = (long long)H * a->hd;
   if (!q || !out || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) || ld_q % 8 || ld_o % 8 || ld_q < width || ld_o < width) return -4;
-  if (H > 65535 || a->B > 65535) return -3;
-  const dim3 grid((a->max_new + 3) / 4, H, a->B);
-#define CALL(T, HD) GB_PDL_LAUNCH((paged_attn_kernel<T, HD>), grid, dim3(128), st, *a, (const T*)q, ld_q, H, scale, window, (T*)out, ld_o)
-  if (a->is_bf16) {
-    if (a->hd == 32) { CALL(__nv_bfloat16, 32); } else if (a->hd == 64) { CALL(__nv_bfloat16, 64); } else { CALL(__nv_bfloat16, 128); }
-  } else {
-    if (a->hd == 32) { CALL(__half, 32); } else if (a->hd == 64) { CALL(__half, 64); } else { CALL(__half, 128); }
-  }
+  const long long need = gb_paged_attn_ws(a, H, window);
+  if (need > 0 && (!ws || ws_floats < need || (reinterpret_cast<uintptr_t>(ws) & 15))) return -5;
+  const PgAttn p = {*a, q, ld_q, H, scale * 1.4426950408889634f, window, out, ld_o, ws};
+  const bool few = (long long)a->max_new * (H / a->KV) <= PG_TOKEN_ROWS;
+  for (int b0 = 0; b0 < a->B; b0 += PG_MOST_SEQS) {
+    const PgAttn s = gb_paged_some(p, b0);
+    int rc = 0;
+    if (few) {
+      rc = pg_token_attn(s, st);
+    } else {
+      const dim3 grid((a->max_new + 3) / 4, H, s.a.B);
+#define CALL(T, HD) GB_PDL_LAUNCH((paged_attn_kernel<T, HD>), grid, dim3(128), st, s.a, (const T*)s.q, ld_q, H, scale, window, (T*)s.out, ld_o)
+      if (a->is_bf16) {
+        if (a->hd == 32) { CALL(__nv_bfloat16, 32); } else if (a->hd == 64) { CALL(__nv_bfloat16, 64); } else { CALL(__nv_bfloat16, 128); }
+      } else {
+        if (a->hd == 32) { CALL(__half, 32); } else if (a->hd == 64) { CALL(__half, 64); } else { CALL(__half, 128); }
+      }
 #undef CALL
-  return gb_launch_rc();
+      rc = gb_launch_rc();
+    }
+    if (rc) return rc;
+  }
+  return 0;
 }

@@ -1,0 +1,537 @@
+// Attention over the paged 8-bit cache for few query rows a key head (interface in gb_paged.h, choice in paged_attn.cu): a token or some proposed ones a sequence.
+//
+// Bound by the bytes of the codes, so the work is cut by pages, not by sequences: all (sequence, key head, page) in a row are dealt to the GPU's warps in equal runs, whatever the
+// lengths are (mode "balanced"; the lengths are on the device and so is the dealing).  A warp streams its run through a ring of its own in shared memory, a bulk copy a
+// page of keys or values (4 KB at hd 64), and waits for nobody until its run is over: pieces of a (sequence, head) that lie in one warp are finished there, the others are joined
+// first in the block, then, across blocks, by a second kernel.  Where all items have a block each and few pages, a block takes an item and nothing is left to join (mode "item").
+//
+// A page is two products on the legacy tensor path, with the codes as float16 integers (exact): keys x queries and values x weights, so that
+// queries (8 columns) rather than keys are padded; 16 rows of queries would pad 3 of them to 16.  The order of the contracted dimensions is free as long as both operands have the
+// same, so a lane takes 16 consecutive bytes of a key, or of a value's tokens, and these are its MMA fragments.  The page's key scale joins the score's factor and its value
+// scale the exponent of the weights: w = 2^(s - m + 15 + e - E), with m the running maximum, e the value scale's exponent and E the largest so far.  Rounded to float16 a
+// weight is off by 2^-12 of itself, or by 2^-39 of the largest page's, whichever is more; the row sum has the unrounded weights.  Queries are scaled by a power of two so that a
+// row's largest is between 2^14 and 2^15: float16 then holds them as exactly as bfloat16 does.
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace gb {
+
+constexpr int TK_WARPS = 8, TK_THREADS = 32 * TK_WARPS;
+constexpr int TK_ITEM_PAGES = 16;            // most pages a sequence may show in mode "item"
+constexpr float TK_OFF = 15.f;               // weights are held as 2^15 of themselves, the most float16 takes
+
+// 4 codes (a little-endian word) as two pairs of float16: the bytes, raised by 128, under the exponent of 1024, which is 1024 + 128 + code
+__device__ __forceinline__ void tk_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 off = __half2half2(__ushort_as_half(0x6480));           // 1152
+  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+  lo = *reinterpret_cast<uint32_t*>(&x);
+  hi = *reinterpret_cast<uint32_t*>(&y);
+}
+
+__device__ __forceinline__ void tk_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tk_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void tk_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <typename F>
+__device__ __forceinline__ void tk_put(const PgAttn& p, int b, int g, const PgSeq& s, int r, int d, F v) {
+  const int G = p.H / p.a.KV, i = r / G;
+  const long long at = (long long)(s.first + i) * p.ld_o + (long long)(g * G + r - i * G) * p.a.hd + d;
+  if (p.a.is_bf16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(v);
+}
+
+// Pages of sequence b that its queries see: from page `lo`, `n` of them.
+struct TkPages { int lo, n; };
+__device__ __forceinline__ TkPages tk_pages(const PgAttn& p, const PgSeq& s) {
+  if (s.n == 0) return {0, 0};
+  const int lo = p.window > 0 ? max(0, s.start - p.window + 1) / PG : 0;
+  return {lo, (s.start + s.n - 1) / PG - lo + 1};
+}
+
+// One record of an item's piece: R x HD results, then R pairs (maximum, sum)
+template <int HD> __host__ __device__ constexpr int tk_record(int R) { return R * (HD + 2); }
+
+template <int HD, int NQ>
+__global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid_constant__ PgAttn p, int R, int slots, int item_mode) {
+  constexpr int SLOT = PG * HD, KK = HD / 16, VW = HD / 4 < 16 ? HD / 4 : 16, WPC = VW / 4;   // bytes of a lane's chunk of a key, words of it
+  extern __shared__ __align__(128) uint8_t smem[];
+  const gb_paged& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const int rec_n = tk_record<HD>(R);
+  uint8_t* ring = smem + (size_t)warp * slots * SLOT;
+  float* heads = reinterpret_cast<float*>(smem + (size_t)TK_WARPS * slots * SLOT);            // records of the warps' first items
+  uint64_t* bars = reinterpret_cast<uint64_t*>(heads + (TK_WARPS * rec_n + 1) / 2 * 2);
+  int* cut = reinterpret_cast<int*>(bars + TK_WARPS * slots);                                 // items of the warps' records, -1: none
+  volatile int* abort_flag = cut + 2 * TK_WARPS;
+  int* scan = cut + 2 * TK_WARPS + 1;                                                         // sums of the warps
+  int* cum = scan + TK_WARPS + 1;                                                             // pages of the sequences before
+  uint64_t* bar = bars + warp * slots;
+
+  pdl_wait();
+  if (lane == 0) {
+    for (int s = 0; s < slots; ++s) mbar_init(&bar[s], 1);
+    cut[2 * warp] = cut[2 * warp + 1] = -1;
+    if (warp == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
+  // the run of this block: items [ib, ...) of `KVs` heads, pages [c_lo, c_hi) of them all, `quota` a warp
+  const int KVs = item_mode ? 1 : a.KV, b_base = item_mode ? (int)blockIdx.x / a.KV : 0, g_base = item_mode ? (int)blockIdx.x % a.KV : 0;
+  const int nb = item_mode ? 1 : a.B;
+  if (item_mode) {
+    if (threadIdx.x == 0) {
+      cum[0] = 0;
+      cum[1] = tk_pages(p, pg_seq(a, b_base)).n;
+    }
+    __syncthreads();
+  } else {
+    int before = 0;
+    for (int b0 = 0; b0 < nb; b0 += TK_THREADS) {
+      const int b = b0 + (int)threadIdx.x;
+      int v = b < nb ? tk_pages(p, pg_seq(a, b)).n : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (lane == 31) scan[warp] = v;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < TK_WARPS; ++w) {
+        if (w < warp) v += scan[w];
+        all += scan[w];
+      }
+      if (b < nb) cum[b + 1] = before + v;
+      before += all;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) cum[0] = 0;
+    __syncthreads();
+  }
+  const int T = KVs * cum[nb];
+  const int blocks = item_mode ? 1 : (int)gridDim.x, quota = max(1, (T + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
+  const int c_lo = item_mode ? 0 : min(T, (int)blockIdx.x * TK_WARPS * quota), c_hi = min(T, c_lo + TK_WARPS * quota);
+  const int w_lo = min(c_hi, c_lo + warp * quota), w_hi = min(c_hi, w_lo + quota);
+  auto seq_of = [&](int f) {                  // the sequence whose pages hold place f
+    int lo = 0, hi = nb;                      // cum[lo] * KVs <= f < cum[hi] * KVs
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cum[mid] * KVs <= f) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
+
+  uint32_t qf[NQ][KK][2];
+  float qs[NQ][2], m[NQ][2], l[NQ][2], o[NQ][KK][4];
+  int E = -1000, item = -1, pos0 = 0, n_new = 0, f_begin = 0, f_end = 0;
+  PgSeq sq{0, 0, 0};
+
+  auto load_queries = [&](int b, int g) {
+    const int G = p.H / a.KV;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int r = 8 * q + gq, i = r / G;
+      const bool on = r < sq.n * G;
+      float x[HD / 4];
+      uint32_t top = 0;
+      const long long row = (long long)(sq.first + (on ? i : 0)) * p.ld_q + (long long)(g * G + (on ? r - i * G : 0)) * HD;
+#pragma unroll
+      for (int c = 0; c < HD / 4 / VW; ++c) {
+#pragma unroll
+        for (int k = 0; k < VW; k += 8) {
+          if (a.is_bf16) pg_load8(reinterpret_cast<const __nv_bfloat16*>(p.q) + row + 64 * c + tq * VW + k, x + c * VW + k);
+          else pg_load8(reinterpret_cast<const __half*>(p.q) + row + 64 * c + tq * VW + k, x + c * VW + k);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < HD / 4; ++k) {
+        if (!on) x[k] = 0.f;
+        top = max(top, __float_as_uint(fabsf(x[k])));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^14 / (power of two of the largest), and its inverse; a row with a number that is not finite gives NaN
+      const int e = top == 0 ? 127 : min(max(254 + 14 - (int)(top >> 23), 1), 253);
+      const float mul = __uint_as_float((uint32_t)e << 23), inv = __uint_as_float((uint32_t)(254 - e) << 23);
+      const float f = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : inv * p.scale2;
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        const float* y = x + k * 4;
+        qf[q][k][0] = Cvt<__half>::pack2(y[0] * mul, y[1] * mul);
+        qf[q][k][1] = Cvt<__half>::pack2(y[2] * mul, y[3] * mul);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {           // the factor where scores have it: lanes of queries 2t, 2t + 1
+        qs[q][c] = __shfl_sync(0xffffffffu, f, (2 * tq + c) * 4);
+        m[q][c] = -1e30f;
+        l[q][c] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < KK; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[q][k][c] = 0.f;
+    }
+    E = -1000;
+  };
+
+  // the piece at hand is over: to the output where it is the whole item, else into a record
+  auto finish = [&]() {
+    if (item < 0) return;
+    const int b = b_base + item / KVs, g = g_base + item % KVs, rows = sq.n * (p.H / a.KV);
+    const bool whole = f_begin >= w_lo && f_end <= w_hi, first = f_begin <= w_lo;
+    float* rec = first ? heads + warp * rec_n : reinterpret_cast<float*>(ring);
+    const float unit = E < -500 ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float s = l[q][c];
+        s += __shfl_xor_sync(0xffffffffu, s, 4);
+        s += __shfl_xor_sync(0xffffffffu, s, 8);
+        s += __shfl_xor_sync(0xffffffffu, s, 16);
+        const float f = s == 0.f ? 0.f : unit / s;
+        const int r = 8 * q + 2 * tq + c;
+        if (r < rows) {
+#pragma unroll
+          for (int k = 0; k < KK; ++k) {
+            const float u = o[q][k][c] * f, v = o[q][k][2 + c] * f;
+            if (whole) {
+              tk_put(p, b, g, sq, r, 16 * k + gq, u);
+              tk_put(p, b, g, sq, r, 16 * k + gq + 8, v);
+            } else {
+              rec[r * HD + 16 * k + gq] = u;
+              rec[r * HD + 16 * k + gq + 8] = v;
+            }
+          }
+          if (!whole && gq == 0) { rec[R * HD + 2 * r] = m[q][c]; rec[R * HD + 2 * r + 1] = s; }
+        }
+      }
+    }
+    if (!whole && lane == 0) cut[2 * warp + (first ? 0 : 1)] = item;
+    __syncwarp();
+  };
+
+  int slot_in = 0, slot_out = 0;
+  uint32_t parity = 0;
+  for (int base = w_lo; base < w_hi; base += 32) {
+    const int cnt = min(32, w_hi - base);
+    // lane i looks up page i of the batch
+    int u_b = 0, u_g = 0, u_p = 0, u_id = 0, u_f = 0, u_np = 1;
+    float u_ks = 1.f, u_vs = 1.f;
+    bool u_bad = false;
+    if (lane < cnt) {
+      const int f = base + lane;
+      u_b = seq_of(f);
+      u_np = cum[u_b + 1] - cum[u_b];
+      const int local = f - cum[u_b] * KVs;
+      u_g = local / u_np;
+      u_f = cum[u_b] * KVs + u_g * u_np;      // where its item begins
+      const PgSeq s = pg_seq(a, b_base + u_b);
+      u_p = tk_pages(p, s).lo + local - u_g * u_np;
+      u_id = pg_page(a, b_base + u_b, u_p);
+      u_bad = u_id < 0;
+      if (u_bad) u_id = 0;
+      const long long at = (long long)u_id * a.KV + g_base + u_g;
+      if (!u_bad) { u_ks = a.ks[at]; u_vs = a.vs[at]; }
+    }
+    const unsigned bad = __ballot_sync(0xffffffffu, u_bad);
+    auto issue = [&](int h) {                 // half h of the batch: keys (even) or values of page h / 2
+      const int id = __shfl_sync(0xffffffffu, u_id, h >> 1), g = g_base + __shfl_sync(0xffffffffu, u_g, h >> 1);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar[slot_in], SLOT);
+        tk_bulk(ring + slot_in * SLOT, ((h & 1) ? a.v : a.k) + ((long long)id * a.KV + g) * SLOT, SLOT, &bar[slot_in]);
+      }
+      slot_in = slot_in + 1 == slots ? 0 : slot_in + 1;
+    };
+    auto next = [&]() {
+      if (++slot_out == slots) { slot_out = 0; parity ^= 1u; }
+    };
+    for (int h = 0; h < min(slots, 2 * cnt); ++h) issue(h);
+    for (int i = 0; i < cnt; ++i) {
+      const int f0 = __shfl_sync(0xffffffffu, u_f, i), pg = __shfl_sync(0xffffffffu, u_p, i);
+      const int ub = __shfl_sync(0xffffffffu, u_b, i), ug = __shfl_sync(0xffffffffu, u_g, i), it = ub * KVs + ug;
+      if (it != item) {
+        finish();
+        item = it;
+        f_begin = f0;
+        f_end = f0 + __shfl_sync(0xffffffffu, u_np, i);
+        sq = pg_seq(a, b_base + ub);
+        pos0 = sq.start;
+        n_new = sq.n;
+        load_queries(b_base + ub, g_base + ug);
+      }
+      const float ks = __shfl_sync(0xffffffffu, u_ks, i), vs = __shfl_sync(0xffffffffu, u_vs, i);
+      const bool all_bad = (bad >> i) & 1u;
+      // ---- scores: s[q][j]: keys kA, kA + 2 of key tile j (16 keys), queries 2t, 2t + 1
+      float s[NQ][4][4];
+      wait_or_report(&bar[slot_out], parity, a.status, ST_TIMEOUT_FULL, abort_flag);
+      const uint8_t* sk = ring + slot_out * SLOT + tq * VW;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int kA = 16 * (gq >> 1) + 4 * j + (gq & 1);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[q][j][c] = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < HD / 4 / VW; ++ch) {
+          uint32_t ra[WPC], rb[WPC];
+          if constexpr (WPC == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(sk + kA * HD + 64 * ch), y = *reinterpret_cast<const uint4*>(sk + (kA + 2) * HD + 64 * ch);
+            ra[0] = x.x; ra[1] = x.y; ra[2] = x.z; ra[3] = x.w;
+            rb[0] = y.x; rb[1] = y.y; rb[2] = y.z; rb[3] = y.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(sk + kA * HD), y = *reinterpret_cast<const uint2*>(sk + (kA + 2) * HD);
+            ra[0] = x.x; ra[1] = x.y;
+            rb[0] = y.x; rb[1] = y.y;
+          }
+#pragma unroll
+          for (int w = 0; w < WPC; ++w) {
+            uint32_t a0, a1, a2, a3;
+            tk_halves(ra[w], a0, a2);
+            tk_halves(rb[w], a1, a3);
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) tk_mma(s[q][j], a0, a1, a2, a3, qf[q][ch * WPC + w][0], qf[q][ch * WPC + w][1]);
+          }
+        }
+      }
+      __syncwarp();
+      next();
+      if (2 * i + slots < 2 * cnt) issue(2 * i + slots);
+      // ---- weights
+      const bool edge = all_bad || (pg + 1) * PG > pos0 + 1 || (p.window > 0 && pg * PG <= pos0 + n_new - 1 - p.window);
+      float f[NQ][2];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        f[q][0] = qs[q][0] * ks;
+        f[q][1] = qs[q][1] * ks;
+      }
+      if (edge) {
+        const int G = p.H / a.KV;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int pos = pos0 + (8 * q + 2 * tq + c) / G;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = pg * PG + 16 * (gq >> 1) + 4 * j + (gq & 1) + 2 * e;
+                const bool see = !all_bad && key <= pos && (p.window <= 0 || key > pos - p.window);
+                s[q][j][2 * e + c] = see ? s[q][j][2 * e + c] * f[q][c] : -INFINITY;
+              }
+            f[q][c] = 1.f;
+          }
+      }
+      const int ev = (int)(__float_as_uint(vs) >> 23) - 127, En = max(E, ev);
+      const float shrink = E == En ? 1.f : exp2f((float)(E - En));
+      const float de = fmaxf((float)(ev - En), -60.f), up = exp2f(-de);
+      bool same = E == En;
+      uint32_t pb[NQ][4][2];
+      float corr[NQ][2];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float mn[2], sum[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = fmaxf(fmaxf(fmaxf(s[q][0][c], s[q][0][2 + c]), fmaxf(s[q][1][c], s[q][1][2 + c])),
+                          fmaxf(fmaxf(s[q][2][c], s[q][2][2 + c]), fmaxf(s[q][3][c], s[q][3][2 + c])));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          mn[c] = fmaxf(m[q][c], x * f[q][c]);
+          corr[q][c] = pg_ex2(m[q][c] - mn[c]);
+          same = same && mn[c] == m[q][c];
+          m[q][c] = mn[c];
+          sum[c] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float w0 = pg_ex2(fmaf(s[q][j][2 * e], f[q][0], TK_OFF + de - mn[0]));
+            const float w1 = pg_ex2(fmaf(s[q][j][2 * e + 1], f[q][1], TK_OFF + de - mn[1]));
+            sum[0] += w0;
+            sum[1] += w1;
+            pb[q][j][e] = tk_transpose(Cvt<__half>::pack2(w0, w1));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          l[q][c] = fmaf(l[q][c], corr[q][c], sum[c] * up);
+          corr[q][c] *= shrink;
+        }
+      }
+      E = En;
+      if (__any_sync(0xffffffffu, !same)) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[q][k][c] *= corr[q][c & 1];
+      }
+      // ---- values: o[q][k]: dimensions 16k + g, 16k + g + 8, queries 2t, 2t + 1
+      wait_or_report(&bar[slot_out], parity, a.status, ST_TIMEOUT_FULL, abort_flag);
+      const uint8_t* sv = ring + slot_out * SLOT + tq * 16;
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        const uint4 x = *reinterpret_cast<const uint4*>(sv + (16 * k + gq) * PG), y = *reinterpret_cast<const uint4*>(sv + (16 * k + gq + 8) * PG);
+        const uint32_t ra[4] = {x.x, x.y, x.z, x.w}, rb[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a0, a1, a2, a3;
+          tk_halves(ra[j], a0, a2);
+          tk_halves(rb[j], a1, a3);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) tk_mma(o[q][k], a0, a1, a2, a3, pb[q][j][0], pb[q][j][1]);
+        }
+      }
+      __syncwarp();
+      next();
+      if (2 * i + 1 + slots < 2 * cnt) issue(2 * i + 1 + slots);
+    }
+  }
+  finish();
+  __syncthreads();
+
+  // ---- pieces of the block's warps, in order; neighbours of one item are joined
+  auto rec_of = [&](int k) { return (k & 1) ? reinterpret_cast<const float*>(smem + (size_t)(k >> 1) * slots * SLOT) : heads + (k >> 1) * rec_n; };
+  for (int k0 = 0; k0 < 2 * TK_WARPS;) {
+    const int it = cut[k0];
+    int k1 = k0 + 1;
+    if (it >= 0) {
+      while (k1 < 2 * TK_WARPS && (cut[k1] < 0 || cut[k1] == it)) ++k1;
+      const int b = it / KVs, g = it % KVs, np = cum[b + 1] - cum[b], f0 = cum[b] * KVs + g * np;
+      const bool whole = f0 >= c_lo && f0 + np <= c_hi;
+      const PgSeq s = pg_seq(a, b_base + b);
+      const int rows = s.n * (p.H / a.KV);
+      float* part = p.part + (size_t)(2 * blockIdx.x + (f0 > c_lo ? 1 : 0)) * rec_n;
+      for (int i = threadIdx.x; i < rows * HD; i += TK_THREADS) {
+        const int r = i / HD, d = i - r * HD;
+        float top = -1e30f, sum = 0.f, acc = 0.f;
+        for (int k = k0; k < k1; ++k)
+          if (cut[k] >= 0) top = fmaxf(top, rec_of(k)[R * HD + 2 * r]);
+        for (int k = k0; k < k1; ++k)
+          if (cut[k] >= 0) {
+            const float* rec = rec_of(k);
+            const float w = rec[R * HD + 2 * r + 1] == 0.f ? 0.f : rec[R * HD + 2 * r + 1] * pg_ex2(rec[R * HD + 2 * r] - top);
+            sum += w;
+            acc += w == 0.f ? 0.f : w * rec[i];
+          }
+        const float v = sum == 0.f ? 0.f : acc / sum;
+        if (whole) {
+          tk_put(p, b_base + b, g_base + g, s, r, d, v);
+        } else {
+          part[i] = v;
+          if (d == 0) { part[R * HD + 2 * r] = top; part[R * HD + 2 * r + 1] = sum; }
+        }
+      }
+    }
+    k0 = k1;
+  }
+}
+
+// Joins what blocks left of an item: one block a (row, key head, sequence).
+template <int HD>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PgAttn p, int R, int blocks) {
+  __shared__ int red[2][4];
+  __shared__ float part_sum[128], part_acc[128];
+  const gb_paged& a = p.a;
+  const int r = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  // starts and counts are older than the launch ahead, which is past its own wait: only its records are waited for
+  int before = 0, total = 0;
+  for (int i = threadIdx.x; i < a.B; i += 128) {
+    const int n = tk_pages(p, pg_seq(a, i)).n;
+    total += n;
+    if (i < b) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = before; red[1][threadIdx.x >> 5] = total; }
+  pdl_wait();
+  __syncthreads();
+  before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+  const int T = a.KV * (red[1][0] + red[1][1] + red[1][2] + red[1][3]);
+  const PgSeq s = pg_seq(a, b);
+  const int np = tk_pages(p, s).n, G = p.H / a.KV;
+  if (np == 0 || r >= s.n * G) return;
+  const int span = TK_WARPS * max(1, (T + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
+  const int f0 = a.KV * before + g * np, c0 = f0 / span, c1 = (f0 + np - 1) / span;
+  if (c0 == c1) return;                              // one block had all of it
+  const int rec_n = tk_record<HD>(R), d = threadIdx.x % HD, k = threadIdx.x / HD;
+  auto rec_of = [&](int c) { return p.part + (size_t)(2 * c + (f0 > c * span ? 1 : 0)) * rec_n; };
+  float top = -1e30f, sum = 0.f, acc = 0.f;
+  for (int c = c0; c <= c1; ++c) top = fmaxf(top, rec_of(c)[R * HD + 2 * r]);
+  for (int c = c0 + k; c <= c1; c += 128 / HD) {
+    const float* rec = rec_of(c);
+    const float l = rec[R * HD + 2 * r + 1], w = l == 0.f ? 0.f : l * pg_ex2(rec[R * HD + 2 * r] - top);
+    sum += w;
+    acc += w == 0.f ? 0.f : w * rec[r * HD + d];
+  }
+  part_sum[threadIdx.x] = sum;
+  part_acc[threadIdx.x] = acc;
+  __syncthreads();
+  if (threadIdx.x < HD) {
+    for (int j = 1; j < 128 / HD; ++j) { sum += part_sum[threadIdx.x + j * HD]; acc += part_acc[threadIdx.x + j * HD]; }
+    tk_put(p, b, g, s, r, d, sum == 0.f ? 0.f : acc / sum);
+  }
+}
+
+// Pages of a sequence that can be visible, at most
+static int tk_most_pages(const PgAttn& p) {
+  if (p.window <= 0) return p.a.W;
+  return (int)std::min<long long>(p.a.W, ((long long)p.window + p.a.max_new + 2 * PG - 3) / PG);
+}
+static bool tk_item_mode(const PgAttn& p) { return (long long)p.a.B * p.a.KV <= pg_sms() && tk_most_pages(p) <= TK_ITEM_PAGES; }
+
+constexpr size_t TK_SMEM = 227 * 1024;
+
+template <int HD, int NQ>
+static int tk_go(const PgAttn& p, int R, cudaStream_t st) {
+  const int item = tk_item_mode(p);
+  const size_t fixed = ((size_t)TK_WARPS * tk_record<HD>(R) * 4 + 15) / 16 * 16 + (3 * TK_WARPS + 2 + (item ? 1 : p.a.B) + 1) * 4 + 16;
+  constexpr int most = HD == 32 ? 8 : HD == 64 ? 5 : 3;
+  const int slots = (int)std::min<size_t>(most, (TK_SMEM - fixed) / (TK_WARPS * ((size_t)PG * HD + 8)));
+  if (slots < 2) return -3;
+  const size_t smem = fixed + (size_t)slots * TK_WARPS * (PG * HD + 8);
+  const int blocks = item ? p.a.B * p.a.KV : pg_sms();
+  GB_PDL_LAUNCH_SMEM((paged_token_kernel<HD, NQ>), dim3(blocks), dim3(TK_THREADS), smem, st, p, R, slots, item);
+  const int rc = gb_launch_rc();
+  if (rc || item) return rc;
+  GB_PDL_LAUNCH((paged_join_kernel<HD>), dim3(R, p.a.KV, p.a.B), dim3(128), st, p, R, blocks);
+  return gb_launch_rc();
+}
+
+template <int HD>
+static int tk_size(const PgAttn& p, int R, cudaStream_t st) { return R <= 8 ? tk_go<HD, 1>(p, R, st) : tk_go<HD, 2>(p, R, st); }
+
+long long pg_token_ws(const PgAttn& p) {
+  const int R = (int)(p.a.max_new * (p.H / p.a.KV));
+  return tk_item_mode(p) ? 0 : 2ll * pg_sms() * R * (p.a.hd + 2);
+}
+
+int pg_token_attn(const PgAttn& p, cudaStream_t st) {
+  const int R = p.a.max_new * (p.H / p.a.KV);
+  return p.a.hd == 32 ? tk_size<32>(p, R, st) : p.a.hd == 64 ? tk_size<64>(p, R, st) : tk_size<128>(p, R, st);
+}
+
+}  // namespace gb

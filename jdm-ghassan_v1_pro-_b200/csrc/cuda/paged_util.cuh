@@ -65,6 +65,7 @@ __device__ __forceinline__ void pg_store8(T* p, const float* v) {
 // 0, or why these arguments are refused (the codes of gb_paged.h's launchers)
 static inline int gb_paged_check(const gb_paged* a) {
   if (!a || !a->k || !a->ks || !a->v || !a->vs || !a->status || (a->B > 0 && (!a->table || !a->start))) return -1;
+  if (!a->first != !a->count) return -1;
   if (a->hd != 32 && a->hd != 64 && a->hd != 128) return -2;
   if (a->KV <= 0 || a->pages <= 0 || a->W <= 0 || a->B < 0 || a->max_new < 0 || a->rows < 0) return -3;
   if ((long long)a->W * GB_PAGE > 0x7fffffffll - 4096 || a->max_new > a->W * GB_PAGE || a->rows > 0x7fffffffll) return -3;

@@ -56,7 +56,9 @@ def _protos():
         P = ctypes.POINTER(PagedArgs)
         L.gb_paged_append.argtypes = [P, c_vp, c_ll, c_int, c_vp, c_ll, c_vp, c_vp, c_float, c_vp, c_int, c_int, c_vp]
         L.gb_paged_read.argtypes = [P, c_vp, c_ll, c_vp, c_ll, c_vp]
-        L.gb_paged_attn.argtypes = [P, c_vp, c_ll, c_int, c_float, c_int, c_vp, c_ll, c_vp]
+        L.gb_paged_attn.argtypes = [P, c_vp, c_ll, c_int, c_float, c_int, c_vp, c_ll, c_vp, c_ll, c_vp]
+        L.gb_paged_attn_ws.argtypes = [P, c_int, c_int]
+        L.gb_paged_attn_ws.restype = c_ll
         _proto = L
     return _proto
 
@@ -149,10 +151,10 @@ def append(pages: Pages, qkv, table, start, max_new: int, cos_sin, H: int, *, fi
     return q_out
 
 
-def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, window: int = 0, first=None, count=None, out=None):
+def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, window: int = 0, first=None, count=None, out=None, scratch=None):
     """Attention of the new tokens' queries ``q`` [rows, H * hd] over the pages, which hold the new tokens' keys already (:func:`append` with the same
     ``start``): each sees the tokens up to its own place, the last ``window`` of them where that is not 0.  Rows of no sequence are not
-    written (without ``out`` they hold anything)."""
+    written (without ``out`` they hold anything).  ``scratch``: float32, :func:`attn_scratch` numbers, one call's at a time; without it the call allocates its own."""
     KV, hd, dev = pages.k.shape[1], pages.k.shape[3], pages.k.device
     if H < 1 or H % KV:
         raise ValueError(f"paged attention: {H} query heads for {KV} key heads")
@@ -161,9 +163,28 @@ def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, w
     _rows(q, H * hd, q.dtype, dev, "paged attention")
     out = _out(out, q.shape[0], H * hd, q.dtype, dev, "paged attention")
     a = _args(pages, table, start, max_new, first, count, q.shape[0], q.dtype, "paged attention")
-    rc = _protos().gb_paged_attn(ctypes.byref(a), q.data_ptr(), q.stride(0), H, scale, window, out.data_ptr(), out.stride(0), _lib.stream_ptr())
+    L = _protos()
+    need = L.gb_paged_attn_ws(ctypes.byref(a), H, window)
+    if need > 0 and scratch is None:
+        scratch = torch.empty(need, dtype=torch.float32, device=dev)
+    if need > 0 and (scratch.dtype != torch.float32 or scratch.device != dev or not scratch.is_contiguous() or scratch.numel() < need):
+        raise ValueError(f"paged attention: scratch is {need} contiguous float32 numbers on the pool's device")
+    rc = L.gb_paged_attn(ctypes.byref(a), q.data_ptr(), q.stride(0), H, scale, window, out.data_ptr(), out.stride(0),
+                         scratch.data_ptr() if need > 0 else None, need, _lib.stream_ptr())
     _lib.check_rc(rc, "gb_paged_attn")
     return out
+
+
+def attn_scratch(B: int, width: int, kv_heads: int, head_dim: int, max_new: int, H: int, window: int = 0) -> int:
+    """float32 numbers that :func:`attn` needs for ``B`` sequences with tables of ``width`` pages."""
+    a = PagedArgs()
+    for f in ("k", "ks", "v", "vs", "table", "start", "status"):
+        setattr(a, f, 4096)                                   # sizes alone count
+    a.pages, a.KV, a.hd, a.W, a.B, a.max_new, a.rows = 1, kv_heads, head_dim, width, B, max_new, B * max_new
+    need = _protos().gb_paged_attn_ws(ctypes.byref(a), H, window)
+    if need < 0:
+        _lib.check_rc(int(need), "gb_paged_attn_ws")
+    return int(need)
 
 
 def read(pages: Pages, table, start, max_new: int, dtype, rows: int, *, first=None, count=None, k_out=None, v_out=None):

@@ -82,7 +82,7 @@ def test_the_c_launchers_refuse_before_they_touch_the_device():
     for n, t in (("gb_paged_append", [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
                  ("gb_paged_attn", [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_int,
-                                   ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
+                                   ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
                  ("gb_paged_read", [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p])):
         getattr(L, n).argtypes = t
 
@@ -97,7 +97,7 @@ def test_the_c_launchers_refuse_before_they_touch_the_device():
 
     def three(ptr, x=4096, ldx=512, h=4, out=4096, ldo=256, scale=0.1, window=0, cs=4096, positions=9, rope=0):
         return (L.gb_paged_append(ptr, x, ldx, h, out, ldo, None, None, 1e-6, cs, positions, rope, None),
-                L.gb_paged_attn(ptr, x, ldx, h, scale, window, out, ldo, None), L.gb_paged_read(ptr, out, ldo, out, ldo, None))
+                L.gb_paged_attn(ptr, x, ldx, h, scale, window, out, ldo, None, 0, None), L.gb_paged_read(ptr, out, ldo, out, ldo, None))
 
     assert three(None) == (-1, -1, -1)
     for kw, rc in [(dict(k=None), -1), (dict(status=None), -1), (dict(start=None), -1), (dict(hd=96), -2), (dict(KV=0), -3), (dict(pages=0), -3), (dict(W=0), -3),
@@ -105,6 +105,10 @@ def test_the_c_launchers_refuse_before_they_touch_the_device():
                    (dict(v=4104), -4)]:
         ptr, keep = block(**kw)
         assert three(ptr) == (rc, rc, rc), kw
+    ptr, keep = block(first=4096)
+    assert three(ptr) == (-1, -1, -1)                         # first without count
+    ptr, keep = block(W=4000, B=200)
+    assert three(ptr)[1] == -5                                # no workspace
     ptr, keep = block()
     assert three(ptr, h=3)[:2] == (-1, -1) and three(ptr, x=4098)[:2] == (-4, -4) and three(ptr, out=4098) == (-4, -4, -4) and three(ptr, ldx=504)[0] == -4
     assert three(ptr, ldo=260) == (-4, -4, -4) and three(ptr, scale=0.0)[1] == -1 and three(ptr, window=-1)[1] == -1
