@@ -63,6 +63,7 @@ int pg_sms() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { (void)cudaGetLastError(); return 148; }
   if ((n = known[dev].load(std::memory_order_relaxed))) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { (void)cudaGetLastError(); return 148; }
+  n = std::min(n, PG_MOST_BLOCKS);
   known[dev].store(n, std::memory_order_relaxed);
   return n;
 }

@@ -5,6 +5,7 @@
 namespace gb {
 
 constexpr int PG_TOKEN_ROWS = 16;            // query rows a key head (tokens x heads of a group) up to which the token kernel runs
+constexpr int PG_MOST_BLOCKS = 256;          // blocks that pieces are dealt to, at most
 constexpr int PG_MOST_SEQS = 2048;           // sequences of one launch; more are several launches
 
 struct PgAttn {
@@ -22,7 +23,7 @@ __device__ __forceinline__ float pg_ex2(float x) {
   return r;
 }
 
-int pg_sms();                                // of the current device
+int pg_sms();                                // of the current device, at most PG_MOST_BLOCKS
 long long pg_token_ws(const PgAttn& p);
 int pg_token_attn(const PgAttn& p, cudaStream_t st);
 

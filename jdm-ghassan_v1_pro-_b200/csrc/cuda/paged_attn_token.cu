@@ -46,12 +46,11 @@ __device__ __forceinline__ void tk_bulk(void* dst, const void* src, uint32_t byt
                : "memory");
 }
 
-template <typename F>
-__device__ __forceinline__ void tk_put(const PgAttn& p, int b, int g, const PgSeq& s, int r, int d, F v) {
+// Where row r of (the sequence with rows from `first` on, key head g) goes.
+template <typename T, int HD>
+__device__ __forceinline__ T* tk_out(const PgAttn& p, int first, int g, int r) {
   const int G = p.H / p.a.KV, i = r / G;
-  const long long at = (long long)(s.first + i) * p.ld_o + (long long)(g * G + r - i * G) * p.a.hd + d;
-  if (p.a.is_bf16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-  else reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(v);
+  return reinterpret_cast<T*>(p.out) + (long long)(first + i) * p.ld_o + (long long)(g * G + r - i * G) * HD;
 }
 
 // Pages of sequence b that its queries see: from page `lo`, `n` of them.
@@ -62,10 +61,12 @@ __device__ __forceinline__ TkPages tk_pages(const PgAttn& p, const PgSeq& s) {
   return {lo, (s.start + s.n - 1) / PG - lo + 1};
 }
 
-// One record of an item's piece: R x HD results, then R pairs (maximum, sum)
+// Whose piece a warp left in a record: the item, its places, its sequence's first row, its rows.
+struct TkCut { int item, f0, f1, first, rows; };
+// A record: R x HD results, then R pairs (maximum, sum)
 template <int HD> __host__ __device__ constexpr int tk_record(int R) { return R * (HD + 2); }
 
-template <int HD, int NQ>
+template <typename T, int HD, int NQ>
 __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid_constant__ PgAttn p, int R, int slots, int item_mode) {
   constexpr int SLOT = PG * HD, KK = HD / 16, VW = HD / 4 < 16 ? HD / 4 : 16, WPC = VW / 4;   // bytes of a lane's chunk of a key, words of it
   extern __shared__ __align__(128) uint8_t smem[];
@@ -75,33 +76,42 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   uint8_t* ring = smem + (size_t)warp * slots * SLOT;
   float* heads = reinterpret_cast<float*>(smem + (size_t)TK_WARPS * slots * SLOT);            // records of the warps' first items
   uint64_t* bars = reinterpret_cast<uint64_t*>(heads + (TK_WARPS * rec_n + 1) / 2 * 2);
-  int* cut = reinterpret_cast<int*>(bars + TK_WARPS * slots);                                 // items of the warps' records, -1: none
-  volatile int* abort_flag = cut + 2 * TK_WARPS;
-  int* scan = cut + 2 * TK_WARPS + 1;                                                         // sums of the warps
+  TkCut* cut = reinterpret_cast<TkCut*>(bars + TK_WARPS * slots);                             // what the warps' records are of
+  float* wt = reinterpret_cast<float*>(cut + 2 * TK_WARPS);                                   // their weights, [record][row]
+  int* scan = reinterpret_cast<int*>(wt + 2 * TK_WARPS * 8 * NQ);                             // sums of the warps
+  volatile int* abort_flag = scan + TK_WARPS;
   int* cum = scan + TK_WARPS + 1;                                                             // pages of the sequences before
+  int* lows = cum + (item_mode ? 1 : p.a.B) + 1;                                              // their first visible pages
   uint64_t* bar = bars + warp * slots;
 
-  pdl_wait();
   if (lane == 0) {
     for (int s = 0; s < slots; ++s) mbar_init(&bar[s], 1);
-    cut[2 * warp] = cut[2 * warp + 1] = -1;
+    cut[2 * warp].item = cut[2 * warp + 1].item = -1;
     if (warp == 0) *abort_flag = 0;
     fence_barrier_init();
   }
+  pdl_wait();
   // the run of this block: items [ib, ...) of `KVs` heads, pages [c_lo, c_hi) of them all, `quota` a warp
   const int KVs = item_mode ? 1 : a.KV, b_base = item_mode ? (int)blockIdx.x / a.KV : 0, g_base = item_mode ? (int)blockIdx.x % a.KV : 0;
   const int nb = item_mode ? 1 : a.B;
   if (item_mode) {
     if (threadIdx.x == 0) {
       cum[0] = 0;
-      cum[1] = tk_pages(p, pg_seq(a, b_base)).n;
+      const TkPages v = tk_pages(p, pg_seq(a, b_base));
+      cum[1] = v.n;
+      lows[0] = v.lo;
     }
     __syncthreads();
   } else {
     int before = 0;
     for (int b0 = 0; b0 < nb; b0 += TK_THREADS) {
       const int b = b0 + (int)threadIdx.x;
-      int v = b < nb ? tk_pages(p, pg_seq(a, b)).n : 0;
+      int v = 0;
+      if (b < nb) {
+        const TkPages seen = tk_pages(p, pg_seq(a, b));
+        v = seen.n;
+        lows[b] = seen.lo;
+      }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -122,9 +132,9 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
     if (threadIdx.x == 0) cum[0] = 0;
     __syncthreads();
   }
-  const int T = KVs * cum[nb];
-  const int blocks = item_mode ? 1 : (int)gridDim.x, quota = max(1, (T + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
-  const int c_lo = item_mode ? 0 : min(T, (int)blockIdx.x * TK_WARPS * quota), c_hi = min(T, c_lo + TK_WARPS * quota);
+  const int total = KVs * cum[nb];
+  const int blocks = item_mode ? 1 : (int)gridDim.x, quota = max(1, (total + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
+  const int c_lo = item_mode ? 0 : min(total, (int)blockIdx.x * TK_WARPS * quota), c_hi = min(total, c_lo + TK_WARPS * quota);
   const int w_lo = min(c_hi, c_lo + warp * quota), w_hi = min(c_hi, w_lo + quota);
   auto seq_of = [&](int f) {                  // the sequence whose pages hold place f
     int lo = 0, hi = nb;                      // cum[lo] * KVs <= f < cum[hi] * KVs
@@ -152,10 +162,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
 #pragma unroll
       for (int c = 0; c < HD / 4 / VW; ++c) {
 #pragma unroll
-        for (int k = 0; k < VW; k += 8) {
-          if (a.is_bf16) pg_load8(reinterpret_cast<const __nv_bfloat16*>(p.q) + row + 64 * c + tq * VW + k, x + c * VW + k);
-          else pg_load8(reinterpret_cast<const __half*>(p.q) + row + 64 * c + tq * VW + k, x + c * VW + k);
-        }
+        for (int k = 0; k < VW; k += 8) pg_load8(reinterpret_cast<const T*>(p.q) + row + 64 * c + tq * VW + k, x + c * VW + k);
       }
 #pragma unroll
       for (int k = 0; k < HD / 4; ++k) {
@@ -191,7 +198,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   // the piece at hand is over: to the output where it is the whole item, else into a record
   auto finish = [&]() {
     if (item < 0) return;
-    const int b = b_base + item / KVs, g = g_base + item % KVs, rows = sq.n * (p.H / a.KV);
+    const int rows = sq.n * (p.H / a.KV);
     const bool whole = f_begin >= w_lo && f_end <= w_hi, first = f_begin <= w_lo;
     float* rec = first ? heads + warp * rec_n : reinterpret_cast<float*>(ring);
     const float unit = E < -500 ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23);
@@ -203,25 +210,28 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         s += __shfl_xor_sync(0xffffffffu, s, 4);
         s += __shfl_xor_sync(0xffffffffu, s, 8);
         s += __shfl_xor_sync(0xffffffffu, s, 16);
-        const float f = s == 0.f ? 0.f : unit / s;
+        const float f = s == 0.f ? 0.f : __fdividef(unit, s);
         const int r = 8 * q + 2 * tq + c;
-        if (r < rows) {
+        if (r >= rows) continue;
+        if (whole) {
+          T* dst = tk_out<T, HD>(p, sq.first, g_base + item % KVs, r) + gq;
 #pragma unroll
           for (int k = 0; k < KK; ++k) {
-            const float u = o[q][k][c] * f, v = o[q][k][2 + c] * f;
-            if (whole) {
-              tk_put(p, b, g, sq, r, 16 * k + gq, u);
-              tk_put(p, b, g, sq, r, 16 * k + gq + 8, v);
-            } else {
-              rec[r * HD + 16 * k + gq] = u;
-              rec[r * HD + 16 * k + gq + 8] = v;
-            }
+            dst[16 * k] = Cvt<T>::from_f(o[q][k][c] * f);
+            dst[16 * k + 8] = Cvt<T>::from_f(o[q][k][2 + c] * f);
           }
-          if (!whole && gq == 0) { rec[R * HD + 2 * r] = m[q][c]; rec[R * HD + 2 * r + 1] = s; }
+        } else {
+          float* dst = rec + r * HD + gq;
+#pragma unroll
+          for (int k = 0; k < KK; ++k) {
+            dst[16 * k] = o[q][k][c] * f;
+            dst[16 * k + 8] = o[q][k][2 + c] * f;
+          }
+          if (gq == 0) *reinterpret_cast<float2*>(rec + R * HD + 2 * r) = make_float2(m[q][c], s);
         }
       }
     }
-    if (!whole && lane == 0) cut[2 * warp + (first ? 0 : 1)] = item;
+    if (!whole && lane == 0) cut[2 * warp + (first ? 0 : 1)] = {item, f_begin, f_end, sq.first, rows};
     __syncwarp();
   };
 
@@ -240,8 +250,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
       const int local = f - cum[u_b] * KVs;
       u_g = local / u_np;
       u_f = cum[u_b] * KVs + u_g * u_np;      // where its item begins
-      const PgSeq s = pg_seq(a, b_base + u_b);
-      u_p = tk_pages(p, s).lo + local - u_g * u_np;
+      u_p = lows[u_b] + local - u_g * u_np;
       u_id = pg_page(a, b_base + u_b, u_p);
       u_bad = u_id < 0;
       if (u_bad) u_id = 0;
@@ -410,89 +419,122 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   finish();
   __syncthreads();
 
-  // ---- pieces of the block's warps, in order; neighbours of one item are joined
-  auto rec_of = [&](int k) { return (k & 1) ? reinterpret_cast<const float*>(smem + (size_t)(k >> 1) * slots * SLOT) : heads + (k >> 1) * rec_n; };
-  for (int k0 = 0; k0 < 2 * TK_WARPS;) {
-    const int it = cut[k0];
-    int k1 = k0 + 1;
-    if (it >= 0) {
-      while (k1 < 2 * TK_WARPS && (cut[k1] < 0 || cut[k1] == it)) ++k1;
-      const int b = it / KVs, g = it % KVs, np = cum[b + 1] - cum[b], f0 = cum[b] * KVs + g * np;
-      const bool whole = f0 >= c_lo && f0 + np <= c_hi;
-      const PgSeq s = pg_seq(a, b_base + b);
-      const int rows = s.n * (p.H / a.KV);
-      float* part = p.part + (size_t)(2 * blockIdx.x + (f0 > c_lo ? 1 : 0)) * rec_n;
-      for (int i = threadIdx.x; i < rows * HD; i += TK_THREADS) {
-        const int r = i / HD, d = i - r * HD;
-        float top = -1e30f, sum = 0.f, acc = 0.f;
-        for (int k = k0; k < k1; ++k)
-          if (cut[k] >= 0) top = fmaxf(top, rec_of(k)[R * HD + 2 * r]);
-        for (int k = k0; k < k1; ++k)
-          if (cut[k] >= 0) {
-            const float* rec = rec_of(k);
-            const float w = rec[R * HD + 2 * r + 1] == 0.f ? 0.f : rec[R * HD + 2 * r + 1] * pg_ex2(rec[R * HD + 2 * r] - top);
-            sum += w;
-            acc += w == 0.f ? 0.f : w * rec[i];
-          }
-        const float v = sum == 0.f ? 0.f : acc / sum;
-        if (whole) {
-          tk_put(p, b_base + b, g_base + g, s, r, d, v);
-        } else {
-          part[i] = v;
-          if (d == 0) { part[R * HD + 2 * r] = top; part[R * HD + 2 * r + 1] = sum; }
+  // ---- pieces of the block's warps; those of one item are joined.  Loads are unconditional and picked from afterwards: behind branches each would wait for
+  // the one before (3400 cycles of the block's end, against 1000).
+  auto rec_of = [&](int k) { return reinterpret_cast<const float*>((k & 1) ? smem + (size_t)(k >> 1) * slots * SLOT : reinterpret_cast<const uint8_t*>(heads + (k >> 1) * rec_n)); };
+  constexpr int RECS = 2 * TK_WARPS;
+  {                                                                   // weight of record k in row r against the item's largest maximum
+    const int k = threadIdx.x % RECS, it = cut[k].item;
+    for (int r0 = 0; r0 < R; r0 += TK_THREADS / RECS) {               // as often for every lane: they exchange
+      const int r = min(r0 + (int)threadIdx.x / RECS, R - 1);
+      const float2 ml = *reinterpret_cast<const float2*>(rec_of(k) + R * HD + 2 * r);
+      float top = -1e30f;
+#pragma unroll
+      for (int j = 0; j < RECS; ++j) {
+        const float v = __shfl_sync(0xffffffffu, ml.x, j, RECS);
+        const int of = __shfl_sync(0xffffffffu, it, j, RECS);
+        top = fmaxf(top, of == it ? v : -1e30f);
+      }
+      wt[k * R + r] = it < 0 || ml.y == 0.f ? 0.f : ml.y * pg_ex2(ml.x - top);
+    }
+  }
+  __syncthreads();
+  const int my_item = lane < RECS ? cut[lane].item : -1;
+  unsigned left = __ballot_sync(0xffffffffu, my_item >= 0);
+  while (left) {
+    const int k0 = __ffs(left) - 1;
+    const unsigned same = __ballot_sync(0xffffffffu, my_item == __shfl_sync(0xffffffffu, my_item, k0));
+    const int k1 = 32 - __clz(same);
+    left &= ~same;
+    const TkCut c = cut[k0];
+    const bool whole = c.f0 >= c_lo && c.f1 <= c_hi;
+    const int g = g_base + c.item % KVs;
+    float* part = p.part + (size_t)(2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0)) * rec_n;
+    for (int i = threadIdx.x; i < c.rows * (HD / 2); i += TK_THREADS) {
+      const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
+      float sum = 0.f, u = 0.f, v = 0.f;
+#pragma unroll 4
+      for (int k = k0; k < k1; ++k) {                                 // records of nobody weigh nothing, whatever they hold
+        const float w = wt[k * R + r];
+        const float2 x = *reinterpret_cast<const float2*>(rec_of(k) + r * HD + d);
+        sum += w;
+        u += w == 0.f ? 0.f : w * x.x;
+        v += w == 0.f ? 0.f : w * x.y;
+      }
+      const float f = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+      if (whole) {
+        *reinterpret_cast<uint32_t*>(tk_out<T, HD>(p, c.first, g, r) + d) = Cvt<T>::pack2(u * f, v * f);
+      } else {
+        *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(u * f, v * f);
+        if (d == 0) {
+          float top = -1e30f;
+          for (int k = k0; k < k1; ++k) top = fmaxf(top, cut[k].item >= 0 ? rec_of(k)[R * HD + 2 * r] : -1e30f);
+          *reinterpret_cast<float2*>(part + R * HD + 2 * r) = make_float2(top, sum);
         }
       }
     }
-    k0 = k1;
   }
 }
 
 // Joins what blocks left of an item: one block a (row, key head, sequence).
-template <int HD>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PgAttn p, int R, int blocks) {
+constexpr int TJ_THREADS = 128;
+template <typename T, int HD>
+__global__ void __launch_bounds__(TJ_THREADS) paged_join_kernel(const __grid_constant__ PgAttn p, int R, int blocks) {
   __shared__ int red[2][4];
-  __shared__ float part_sum[128], part_acc[128];
+  __shared__ float top_of[4], wt[PG_MOST_BLOCKS], sums[TJ_THREADS / 32], acc_of[TJ_THREADS];
   const gb_paged& a = p.a;
-  const int r = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
+  const int r = blockIdx.x, g = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // starts and counts are older than the launch ahead, which is past its own wait: only its records are waited for
-  int before = 0, total = 0;
-  for (int i = threadIdx.x; i < a.B; i += 128) {
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < a.B; i += TJ_THREADS) {
     const int n = tk_pages(p, pg_seq(a, i)).n;
-    total += n;
+    all += n;
     if (i < b) before += n;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
   }
-  if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = before; red[1][threadIdx.x >> 5] = total; }
-  pdl_wait();
+  if (lane == 0) { red[0][warp] = before; red[1][warp] = all; }
+  const PgSeq s = pg_seq(a, b);
   __syncthreads();
   before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-  const int T = a.KV * (red[1][0] + red[1][1] + red[1][2] + red[1][3]);
-  const PgSeq s = pg_seq(a, b);
+  const int total = a.KV * (red[1][0] + red[1][1] + red[1][2] + red[1][3]);
   const int np = tk_pages(p, s).n, G = p.H / a.KV;
-  if (np == 0 || r >= s.n * G) return;
-  const int span = TK_WARPS * max(1, (T + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
+  const int span = TK_WARPS * max(1, (total + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
   const int f0 = a.KV * before + g * np, c0 = f0 / span, c1 = (f0 + np - 1) / span;
-  if (c0 == c1) return;                              // one block had all of it
-  const int rec_n = tk_record<HD>(R), d = threadIdx.x % HD, k = threadIdx.x / HD;
+  const bool mine = np > 0 && r < s.n * G && c0 != c1;       // else one block had all of it
+  pdl_wait();
+  if (!mine) return;
+  const int rec_n = tk_record<HD>(R), n = c1 - c0 + 1;
   auto rec_of = [&](int c) { return p.part + (size_t)(2 * c + (f0 > c * span ? 1 : 0)) * rec_n; };
-  float top = -1e30f, sum = 0.f, acc = 0.f;
-  for (int c = c0; c <= c1; ++c) top = fmaxf(top, rec_of(c)[R * HD + 2 * r]);
-  for (int c = c0 + k; c <= c1; c += 128 / HD) {
-    const float* rec = rec_of(c);
-    const float l = rec[R * HD + 2 * r + 1], w = l == 0.f ? 0.f : l * pg_ex2(rec[R * HD + 2 * r] - top);
-    sum += w;
-    acc += w == 0.f ? 0.f : w * rec[r * HD + d];
+  float top = -1e30f;
+  for (int c = threadIdx.x; c < n; c += TJ_THREADS) top = fmaxf(top, rec_of(c0 + c)[R * HD + 2 * r]);
+  top = warp_max(top);
+  if (lane == 0) top_of[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+  float sum = 0.f;
+  for (int c = threadIdx.x; c < n; c += TJ_THREADS) {
+    const float2 ml = *reinterpret_cast<const float2*>(rec_of(c0 + c) + R * HD + 2 * r);
+    wt[c] = ml.y == 0.f ? 0.f : ml.y * pg_ex2(ml.x - top);
+    sum += wt[c];
   }
-  part_sum[threadIdx.x] = sum;
-  part_acc[threadIdx.x] = acc;
+  sum = warp_sum(sum);
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  const int d = threadIdx.x % HD;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int c = threadIdx.x / HD; c < n; c += TJ_THREADS / HD) acc = fmaf(wt[c], rec_of(c0 + c)[r * HD + d], acc);
+  acc_of[threadIdx.x] = acc;
   __syncthreads();
   if (threadIdx.x < HD) {
-    for (int j = 1; j < 128 / HD; ++j) { sum += part_sum[threadIdx.x + j * HD]; acc += part_acc[threadIdx.x + j * HD]; }
-    tk_put(p, b, g, s, r, d, sum == 0.f ? 0.f : acc / sum);
+#pragma unroll
+    for (int j = 1; j < TJ_THREADS / HD; ++j) acc += acc_of[threadIdx.x + j * HD];
+    tk_out<T, HD>(p, s.first, g, r)[d] = Cvt<T>::from_f(sum == 0.f ? 0.f : acc / sum);
   }
 }
 
@@ -505,24 +547,28 @@ static bool tk_item_mode(const PgAttn& p) { return (long long)p.a.B * p.a.KV <= 
 
 constexpr size_t TK_SMEM = 227 * 1024;
 
-template <int HD, int NQ>
+template <typename T, int HD, int NQ>
 static int tk_go(const PgAttn& p, int R, cudaStream_t st) {
-  const int item = tk_item_mode(p);
-  const size_t fixed = ((size_t)TK_WARPS * tk_record<HD>(R) * 4 + 15) / 16 * 16 + (3 * TK_WARPS + 2 + (item ? 1 : p.a.B) + 1) * 4 + 16;
+  const int item = tk_item_mode(p), blocks = item ? p.a.B * p.a.KV : pg_sms();
+  const size_t fixed = ((size_t)TK_WARPS * tk_record<HD>(R) * 4 + 15) / 16 * 16 + 2 * TK_WARPS * (sizeof(TkCut) + 8 * NQ * 4) +
+                       (TK_WARPS + 1 + 2 * (item ? 1 : p.a.B) + 1) * 4;
   constexpr int most = HD == 32 ? 8 : HD == 64 ? 5 : 3;
   const int slots = (int)std::min<size_t>(most, (TK_SMEM - fixed) / (TK_WARPS * ((size_t)PG * HD + 8)));
   if (slots < 2) return -3;
   const size_t smem = fixed + (size_t)slots * TK_WARPS * (PG * HD + 8);
-  const int blocks = item ? p.a.B * p.a.KV : pg_sms();
-  GB_PDL_LAUNCH_SMEM((paged_token_kernel<HD, NQ>), dim3(blocks), dim3(TK_THREADS), smem, st, p, R, slots, item);
+  GB_PDL_LAUNCH_SMEM((paged_token_kernel<T, HD, NQ>), dim3(blocks), dim3(TK_THREADS), smem, st, p, R, slots, item);
   const int rc = gb_launch_rc();
   if (rc || item) return rc;
-  GB_PDL_LAUNCH((paged_join_kernel<HD>), dim3(R, p.a.KV, p.a.B), dim3(128), st, p, R, blocks);
+  GB_PDL_LAUNCH((paged_join_kernel<T, HD>), dim3(R, p.a.KV, p.a.B), dim3(TJ_THREADS), st, p, R, blocks);
   return gb_launch_rc();
 }
 
-template <int HD>
-static int tk_size(const PgAttn& p, int R, cudaStream_t st) { return R <= 8 ? tk_go<HD, 1>(p, R, st) : tk_go<HD, 2>(p, R, st); }
+template <typename T, int HD>
+static int tk_rows(const PgAttn& p, int R, cudaStream_t st) { return R <= 8 ? tk_go<T, HD, 1>(p, R, st) : tk_go<T, HD, 2>(p, R, st); }
+template <typename T>
+static int tk_size(const PgAttn& p, int R, cudaStream_t st) {
+  return p.a.hd == 32 ? tk_rows<T, 32>(p, R, st) : p.a.hd == 64 ? tk_rows<T, 64>(p, R, st) : tk_rows<T, 128>(p, R, st);
+}
 
 long long pg_token_ws(const PgAttn& p) {
   const int R = (int)(p.a.max_new * (p.H / p.a.KV));
@@ -531,7 +577,7 @@ long long pg_token_ws(const PgAttn& p) {
 
 int pg_token_attn(const PgAttn& p, cudaStream_t st) {
   const int R = p.a.max_new * (p.H / p.a.KV);
-  return p.a.hd == 32 ? tk_size<32>(p, R, st) : p.a.hd == 64 ? tk_size<64>(p, R, st) : tk_size<128>(p, R, st);
+  return p.a.is_bf16 ? tk_size<__nv_bfloat16>(p, R, st) : tk_size<__half>(p, R, st);
 }
 
 }  // namespace gb

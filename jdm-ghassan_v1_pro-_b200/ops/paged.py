@@ -75,39 +75,37 @@ def new_pages(pages: int, kv_heads: int, head_dim: int, device) -> Pages:
 
 
 def _args(p: Pages, table, start, max_new, first, count, rows, dtype, what) -> PagedArgs:
-    pages, KV, _, hd = p.k.shape
-    dev = p.k.device
-    if hd not in HEAD_DIMS or p.k.shape[2] != PAGE or p.v.shape != (pages, KV, hd, PAGE) or p.ks.shape != (pages, KV) or p.vs.shape != (pages, KV):
-        raise ValueError(f"{what}: the pool's tensors do not belong together: {tuple(p.k.shape)}, {tuple(p.v.shape)}, {tuple(p.ks.shape)}, {tuple(p.vs.shape)}")
-    if p.k.dtype != torch.int8 or p.v.dtype != torch.int8 or p.ks.dtype != torch.float32 or p.vs.dtype != torch.float32:
+    k, ks, v, vs = p
+    dev = k.device
+    pages, KV, page, hd = k.shape
+    if hd not in HEAD_DIMS or page != PAGE or v.shape != (pages, KV, hd, PAGE) or ks.shape != (pages, KV) or vs.shape != (pages, KV):
+        raise ValueError(f"{what}: the pool's tensors do not belong together: {tuple(k.shape)}, {tuple(v.shape)}, {tuple(ks.shape)}, {tuple(vs.shape)}")
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise ValueError(f"{what}: a pool holds int8 codes and float32 scales")
     if dtype != torch.float16 and dtype != torch.bfloat16:
         raise ValueError(f"{what}: rows are float16 or bfloat16, not {dtype}")
     if table.dim() != 2 or start.dim() != 1 or start.shape[0] != table.shape[0]:
         raise ValueError(f"{what}: table is [B, width] and start [B], got {tuple(table.shape)} and {tuple(start.shape)}")
-    B = table.shape[0]
-    ints = (table, start) if count is None and first is None else (table, start, first, count) if first is not None and count is not None else None
-    if ints is None:
+    B, W = table.shape
+    if (first is None) != (count is None):
         raise ValueError(f"{what}: first and count come together")
-    for t in ints:
+    for t in (table, start) if count is None else (table, start, first, count):
         if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or (t is not table and t.shape != (B,)):
             raise ValueError(f"{what}: table, start, first and count are contiguous int32 tensors on the pool's device, one number a sequence")
-    for t in p:
-        if t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{what}: the pool's tensors are contiguous and on one device")
-    if max_new < 0 or max_new > table.shape[1] * PAGE or (count is None and max_new != 1):
-        raise ValueError(f"{what}: max_new is {max_new}; a table of {table.shape[1]} pages holds {table.shape[1] * PAGE} tokens" +
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and v.device == dev and ks.device == dev and vs.device == dev):
+        raise ValueError(f"{what}: the pool's tensors are contiguous and on one device")
+    if max_new < 0 or max_new > W * PAGE or (count is None and max_new != 1):
+        raise ValueError(f"{what}: max_new is {max_new}; a table of {W} pages holds {W * PAGE} tokens" +
                          (", and without count every sequence has one" if count is None else ""))
     if dev.type != "cuda" or dev.index != torch.cuda.current_device():
         raise ValueError(f"{what}: the pool is on {dev}, which is not the current device")
-    a = PagedArgs()
-    a.k, a.ks, a.v, a.vs = p.k.data_ptr(), p.ks.data_ptr(), p.v.data_ptr(), p.vs.data_ptr()
-    a.pages, a.KV, a.hd, a.table, a.W, a.B = pages, KV, hd, table.data_ptr(), table.shape[1], B
-    a.start, a.max_new, a.rows, a.is_bf16 = start.data_ptr(), max_new, rows, int(dtype == torch.bfloat16)
-    if first is not None:
-        a.first, a.count = first.data_ptr(), count.data_ptr()
-    a.status = _lib.status_word(dev).data_ptr()
-    return a
+    return PagedArgs(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), pages, KV, hd, table.data_ptr(), W, B, start.data_ptr(),
+                     None if first is None else first.data_ptr(), None if count is None else count.data_ptr(), max_new, rows, dtype == torch.bfloat16,
+                     _lib.status_word(dev).data_ptr())
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev.index).cuda_stream
 
 
 def _rows(t, width, dtype, dev, what):
@@ -146,7 +144,7 @@ def append(pages: Pages, qkv, table, start, max_new: int, cos_sin, H: int, *, fi
     a = _args(pages, table, start, max_new, first, count, qkv.shape[0], qkv.dtype, "paged append")
     rc = _protos().gb_paged_append(ctypes.byref(a), qkv.data_ptr(), qkv.stride(0), H, q_out.data_ptr(), q_out.stride(0),
                                    None if qw is None else qw.data_ptr(), None if kw is None else kw.data_ptr(), eps, cos_sin.data_ptr(), cos_sin.shape[0],
-                                   rope_type, _lib.stream_ptr())
+                                   rope_type, _stream(dev))
     _lib.check_rc(rc, "gb_paged_append")
     return q_out
 
@@ -170,7 +168,7 @@ def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, w
     if need > 0 and (scratch.dtype != torch.float32 or scratch.device != dev or not scratch.is_contiguous() or scratch.numel() < need):
         raise ValueError(f"paged attention: scratch is {need} contiguous float32 numbers on the pool's device")
     rc = L.gb_paged_attn(ctypes.byref(a), q.data_ptr(), q.stride(0), H, scale, window, out.data_ptr(), out.stride(0),
-                         scratch.data_ptr() if need > 0 else None, need, _lib.stream_ptr())
+                         scratch.data_ptr() if need > 0 else None, need, _stream(dev))
     _lib.check_rc(rc, "gb_paged_attn")
     return out
 
@@ -194,6 +192,6 @@ def read(pages: Pages, table, start, max_new: int, dtype, rows: int, *, first=No
     k = _out(k_out, rows, KV * hd, dtype, dev, "paged read")
     v = _out(v_out, rows, KV * hd, dtype, dev, "paged read")
     a = _args(pages, table, start, max_new, first, count, rows, dtype, "paged read")
-    rc = _protos().gb_paged_read(ctypes.byref(a), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _lib.stream_ptr())
+    rc = _protos().gb_paged_read(ctypes.byref(a), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _stream(dev))
     _lib.check_rc(rc, "gb_paged_read")
     return k.unflatten(1, (KV, hd)), v.unflatten(1, (KV, hd))
