@@ -1,61 +1,10 @@
-// Attention over the paged 8-bit cache (interface in gb_paged.h): one warp per query head, keys page by page.
+// Attention over the paged 8-bit cache (interface in gb_paged.h): checks of arguments, choice of the kernel.
 #include <algorithm>
 #include <atomic>
 
 #include "paged_attn.cuh"
 
 namespace gb {
-
-// A lane scores two keys of a page, then sums its dimensions of the values over the page's 64 tokens.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ q, long long ld_q, int H, float scale,
-                                                         int window, T* __restrict__ out, long long ld_o) {
-  __shared__ float sq[4][HD], sp[4][PG];
-  pdl_wait();
-  const int wp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z, g = h / (H / a.KV);
-  const PgSeq s = pg_seq(a, b);
-  constexpr int DL = HD / 32;
-  for (int i = blockIdx.x * 4 + wp; i < s.n; i += gridDim.x * 4) {
-    const long long row = s.first + i;
-    const int pos = s.start + i, from = window > 0 ? max(0, pos - window + 1) : 0;
-    for (int d = lane; d < HD; d += 32) sq[wp][d] = Cvt<T>::to_f(q[row * ld_q + (long long)h * HD + d]);
-    __syncwarp();
-    float m = -1e30f, l = 0.f, o[DL] = {};
-    for (int p = from / PG; p <= pos / PG; ++p) {
-      const int id = pg_page(a, b, p);
-      if (id < 0) continue;
-      const long long at = (long long)id * a.KV + g;
-      float x[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int t = lane + 32 * e, key = p * PG + t;
-        float acc = 0.f;
-        for (int d = 0; d < HD; ++d) acc += sq[wp][d] * (float)a.k[(at * PG + t) * HD + d];
-        x[e] = key <= pos && key >= from ? acc * a.ks[at] * scale : -INFINITY;
-      }
-      const float mn = fmaxf(m, warp_max(fmaxf(x[0], x[1]))), corr = __expf(m - mn);
-      float ps = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float w = __expf(x[e] - mn);
-        sp[wp][lane + 32 * e] = w;
-        ps += w;
-      }
-      l = l * corr + warp_sum(ps);
-      m = mn;
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k < DL; ++k) {
-        float acc = 0.f;
-        for (int t = 0; t < PG; ++t) acc += sp[wp][t] * (float)a.v[(at * HD + lane + 32 * k) * PG + t];
-        o[k] = o[k] * corr + acc * a.vs[at];
-      }
-      __syncwarp();
-    }
-#pragma unroll
-    for (int k = 0; k < DL; ++k) out[row * ld_o + (long long)h * HD + lane + 32 * k] = Cvt<T>::from_f(l == 0.f ? 0.f : o[k] / l);
-  }
-}
 
 int pg_sms() {
   static std::atomic<int> known[64];
@@ -92,7 +41,9 @@ static PgAttn gb_paged_some(const PgAttn& p, int b0) {
 static int gb_paged_attn_args(const gb_paged* a, int H, int window) {
   if (const int rc = gb_paged_check(a)) return rc;
   if (H <= 0 || H % a->KV || window < 0 || H > 65535) return -1;
-  if ((long long)std::min(a->B, PG_MOST_SEQS) * a->W * a->KV > 0x7fffffffll) return -3;
+  // places that work is dealt by are counted in 32 bits: pages, or key tiles of every 256 rows
+  const long long items = ((long long)a->max_new * (H / a->KV) + 255) / 256, places = items > 1 ? items * ((a->W + 1) / 2 + 1) : a->W;
+  if ((long long)a->max_new * H > 0x7fffffffll || std::min(a->B, PG_MOST_SEQS) * (double)places * a->KV > 2e9) return -3;
   return 0;
 }
 
@@ -100,8 +51,8 @@ extern "C" long long gb_paged_attn_ws(const gb_paged* a, int H, int window) {
   if (const int rc = gb_paged_attn_args(a, H, window)) return rc;
   if (a->B == 0 || a->max_new == 0 || a->rows == 0) return 0;
   PgAttn p = {*a, nullptr, 0, H, 0.f, window, nullptr, 0, nullptr};
-  if ((long long)a->max_new * (H / a->KV) <= PG_TOKEN_ROWS) return pg_token_ws(gb_paged_some(p, 0));
-  return 0;
+  p = gb_paged_some(p, 0);
+  return (long long)a->max_new * (H / a->KV) <= PG_TOKEN_ROWS ? pg_token_ws(p) : pg_tile_ws(p);
 }
 
 extern "C" int gb_paged_attn(const gb_paged* a, const void* q, long long ld_q, int H, float scale, int window, void* out, long long ld_o,
@@ -117,20 +68,7 @@ extern "C" int gb_paged_attn(const gb_paged* a, const void* q, long long ld_q, i
   const bool few = (long long)a->max_new * (H / a->KV) <= PG_TOKEN_ROWS;
   for (int b0 = 0; b0 < a->B; b0 += PG_MOST_SEQS) {
     const PgAttn s = gb_paged_some(p, b0);
-    int rc = 0;
-    if (few) {
-      rc = pg_token_attn(s, st);
-    } else {
-      const dim3 grid((a->max_new + 3) / 4, H, s.a.B);
-#define CALL(T, HD) GB_PDL_LAUNCH((paged_attn_kernel<T, HD>), grid, dim3(128), st, s.a, (const T*)s.q, ld_q, H, scale, window, (T*)s.out, ld_o)
-      if (a->is_bf16) {
-        if (a->hd == 32) { CALL(__nv_bfloat16, 32); } else if (a->hd == 64) { CALL(__nv_bfloat16, 64); } else { CALL(__nv_bfloat16, 128); }
-      } else {
-        if (a->hd == 32) { CALL(__half, 32); } else if (a->hd == 64) { CALL(__half, 64); } else { CALL(__half, 128); }
-      }
-#undef CALL
-      rc = gb_launch_rc();
-    }
+    const int rc = few ? pg_token_attn(s, st) : pg_tile_attn(s, st);
     if (rc) return rc;
   }
   return 0;

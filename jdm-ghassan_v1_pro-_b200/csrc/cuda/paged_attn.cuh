@@ -1,4 +1,4 @@
-// What the attention kernels of the paged 8-bit cache share (paged_attn.cu, paged_attn_token.cu).
+// What the attention kernels of the paged 8-bit cache share (paged_attn.cu, paged_attn_token.cu, paged_attn_tile.cu).
 #pragma once
 #include "paged_util.cuh"
 
@@ -23,8 +23,20 @@ __device__ __forceinline__ float pg_ex2(float x) {
   return r;
 }
 
+// 4 codes (a little-endian word) as two pairs of float16: the bytes, raised by 128, under the exponent of 1024, which is 1024 + 128 + code
+__device__ __forceinline__ void pg_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 off = __half2half2(__ushort_as_half(0x6480));           // 1152
+  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+  lo = *reinterpret_cast<uint32_t*>(&x);
+  hi = *reinterpret_cast<uint32_t*>(&y);
+}
+
 int pg_sms();                                // of the current device, at most PG_MOST_BLOCKS
 long long pg_token_ws(const PgAttn& p);
 int pg_token_attn(const PgAttn& p, cudaStream_t st);
+long long pg_tile_ws(const PgAttn& p);
+int pg_tile_attn(const PgAttn& p, cudaStream_t st);
 
 }  // namespace gb

@@ -21,16 +21,6 @@ constexpr int TK_WARPS = 8, TK_THREADS = 32 * TK_WARPS;
 constexpr int TK_ITEM_PAGES = 16;            // most pages a sequence may show in mode "item"
 constexpr float TK_OFF = 15.f;               // weights are held as 2^15 of themselves, the most float16 takes
 
-// 4 codes (a little-endian word) as two pairs of float16: the bytes, raised by 128, under the exponent of 1024, which is 1024 + 128 + code
-__device__ __forceinline__ void tk_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t u = w ^ 0x80808080u;
-  const __half2 off = __half2half2(__ushort_as_half(0x6480));           // 1152
-  uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-  __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
-  lo = *reinterpret_cast<uint32_t*>(&x);
-  hi = *reinterpret_cast<uint32_t*>(&y);
-}
-
 __device__ __forceinline__ void tk_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -311,8 +301,8 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
 #pragma unroll
           for (int w = 0; w < WPC; ++w) {
             uint32_t a0, a1, a2, a3;
-            tk_halves(ra[w], a0, a2);
-            tk_halves(rb[w], a1, a3);
+            pg_halves(ra[w], a0, a2);
+            pg_halves(rb[w], a1, a3);
 #pragma unroll
             for (int q = 0; q < NQ; ++q) tk_mma(s[q][j], a0, a1, a2, a3, qf[q][ch * WPC + w][0], qf[q][ch * WPC + w][1]);
           }
@@ -405,8 +395,8 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t a0, a1, a2, a3;
-          tk_halves(ra[j], a0, a2);
-          tk_halves(rb[j], a1, a3);
+          pg_halves(ra[j], a0, a2);
+          pg_halves(rb[j], a1, a3);
 #pragma unroll
           for (int q = 0; q < NQ; ++q) tk_mma(o[q][k], a0, a1, a2, a3, pb[q][j][0], pb[q][j][1]);
         }
