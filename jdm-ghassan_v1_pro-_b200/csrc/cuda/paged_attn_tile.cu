@@ -17,7 +17,7 @@
 
 namespace gb {
 
-constexpr int TL_ROWS = 256, TL_KEYS = 128, TL_THREADS = 13 * 32;
+constexpr int TL_ROWS = 256, TL_KEYS = 128, TL_THREADS = 512;
 constexpr float TL_OFF = 7.f, TL_LAZY = 8.f;   // weights are held as 2^7 of themselves and may grow 2^8 before the sums are rescaled
 
 template <int HD>
@@ -25,11 +25,33 @@ struct Tl {
   static constexpr int PANELS = HD <= 64 ? 1 : 2;             // 64 dimensions each
   static constexpr int Q = 128 * 128 * PANELS, K = 128 * 128 * PANELS, V = 2 * HD * 128, STAGE = K + V;
   static constexpr int STAGES = HD == 128 ? 2 : 3;
+  // columns of tensor memory: scores 0 and 128; at hd 128 the results take the other 256 and weights go over the scores, which then wait for the second product; else
+  // weights have places of their own and the next scores are found while the soft-max is still at work on these
+  static constexpr bool OVER = HD == 128;
+  static constexpr int P0 = OVER ? 0 : 256, P_STEP = OVER ? 128 : 64, O0 = OVER ? 256 : 384;
+  // registers a thread: soft-max, expanding, issuing; launched with 128, so 2 x 128 x S + 128 x (E + I) is at most 65536
+  static constexpr int REGS_S = HD == 128 ? 184 : 192, REGS_E = HD == 128 ? 104 : 88, REGS_I = 40;
   static constexpr int REC = TL_ROWS * (HD + 2);              // floats of a record: [HD / 4][256] four results, then [256] pairs (maximum, sum)
 };
 
 // What a record is of: places of its item, and which it is.  f1 == 0: nothing.
 struct TlDesc { int f0, f1, b, g, qt, quota, pad0, pad1; };
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 tl_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 tl_add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
 
 struct TlItem { int lo, n; };                                 // first key tile, number of them
 __device__ __forceinline__ TlItem tl_item(const PgAttn& p, const PgSeq& s, int G, int qt) {
@@ -69,8 +91,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sKV = smem + 2 * L::Q;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + L::STAGES * L::STAGE);
-  uint64_t *kv_full = bars, *kv_empty = bars + L::STAGES, *s_full = bars + 2 * L::STAGES, *p_ready = s_full + 2, *o_full = s_full + 4, *q_full = s_full + 6;
-  float4* scales = reinterpret_cast<float4*>(bars + 2 * L::STAGES + 8);       // of a stage: key scales of its two pages, value scales; a negative key scale: no page
+  uint64_t *kv_full = bars, *kv_empty = bars + L::STAGES, *s_full = bars + 2 * L::STAGES, *p_ready = s_full + 2, *o_full = s_full + 4, *q_full = s_full + 6, *s_free = s_full + 8;
+  float4* scales = reinterpret_cast<float4*>(bars + 2 * L::STAGES + 10);      // of a stage: key scales of its two pages, value scales; a negative key scale: no page
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scales + L::STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* cum = reinterpret_cast<int*>(tmem_slot + 2);                           // key tiles (of one head) of the sequences before
@@ -79,7 +101,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) { mbar_init(&kv_full[s], 4); mbar_init(&kv_empty[s], 1); }
-    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); }
+    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -152,10 +174,11 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
     }
 
     if (warp < 8) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::REGS_S));
       // ------------------------------------------------------------------------------------------ soft-max: a thread a row
       const int wg = warp >> 2, r = threadIdx.x & 127;
       const uint32_t row = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t tS = tmem + wg * 128 + row, tO = tmem + 256 + wg * HD + row;
+      const uint32_t tS = tmem + wg * 128 + row, tP = tmem + L::P0 + wg * L::P_STEP + row, tO = tmem + L::O0 + wg * HD + row;
       uint8_t* q_at = sQ + wg * L::Q;
       uint32_t kv_it = 0, it = 0;                              // key tiles so far; those of this warpgroup
       bool ok = true;
@@ -209,44 +232,54 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
                 !at_wait(&kv_full[st], (kv_it / L::STAGES) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag)) { ok = false; break; }
             tc_fence_after();
             const float4 sc = scales[st];
+            float x[128];
+            {
+              uint32_t(*rg)[32] = reinterpret_cast<uint32_t(*)[32]>(x);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, rg[c]);
+              tmem_ld_wait();
+            }
+            if constexpr (!L::OVER) {                          // the next scores may come
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_free[wg]);
+            }
             const int base = (item.lo + t) * TL_KEYS;
-            const int hi = pos - base, lo = p.window > 0 ? pos - p.window + 1 - base : 0;
-            const bool mask = base + TL_KEYS - 1 > pos_a || (p.window > 0 && pos_z - p.window + 1 > base) || sc.x < 0.f || sc.y < 0.f;
-            const float f[2] = {qs * sc.x, qs * sc.y};
-            // columns of a half that this row sees
-            const int h_lo[2] = {sc.x < 0.f ? 128 : max(lo, 0), sc.y < 0.f ? 128 : max(lo, 64)}, h_hi[2] = {min(hi, 63), min(hi, 127)};
-            float mt = -INFINITY;
+            if (base + TL_KEYS - 1 > pos_a || (p.window > 0 && pos_z - p.window + 1 > base) || sc.x < 0.f || sc.y < 0.f) {
+              const int hi = pos - base, lo = p.window > 0 ? pos - p.window + 1 - base : 0;
+#pragma unroll
+              for (int k = 0; k < 128; ++k)
+                if (k > hi || k < lo || (k < 64 ? sc.x : sc.y) < 0.f) x[k] = -INFINITY;
+            }
+            // a factor that is too small for fp32 must not make nothing of a hidden score
+            float f[2] = {qs * fabsf(sc.x), qs * fabsf(sc.y)};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) f[h] = f[h] == 0.f ? 1e-37f : f[h];
+            float mt[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float mr[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              float mr[4];
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                uint32_t rg[32];
-                tmem_ld_32x32(tS + h * 64 + c * 32, rg);
-                tmem_ld_wait();
-                if (!mask) {
+              for (int c = 0; c < 4; ++c) mr[c] = fmaxf(x[h * 64 + c], x[h * 64 + 4 + c]);
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) mr[k & 3] = fmaxf(mr[k & 3], __uint_as_float(rg[k]));
-                } else {
+              for (int k = 8; k < 64; k += 8)
 #pragma unroll
-                  for (int k = 0; k < 32; ++k) {
-                    const int j = h * 64 + c * 32 + k;
-                    mr[k & 3] = fmaxf(mr[k & 3], j >= h_lo[h] && j <= h_hi[h] ? __uint_as_float(rg[k]) : -INFINITY);
-                  }
-                }
-              }
-              const float top = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3]));
-              mt = fmaxf(mt, top == -INFINITY ? -INFINITY : top * f[h]);
+                for (int c = 0; c < 4; ++c) mr[c] = fmaxf(fmaxf(mr[c], x[h * 64 + k + c]), x[h * 64 + k + 4 + c]);
+              mt[h] = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3])) * f[h];
             }
+            const float top = fmaxf(mt[0], mt[1]);
             const int e0 = (int)(__float_as_uint(sc.z) >> 23) - 127, e1 = (int)(__float_as_uint(sc.w) >> 23) - 127, En = max(E, max(e0, e1));
-            if (__any_sync(0xffffffffu, mt > m2 + TL_LAZY || En != E)) {
-              const float mn = fmaxf(m2, mt), corr = pg_ex2(m2 - mn);
+            // the last second product is done: its weights' places are free, its sums can be rescaled
+            if (t > k0 && (!L::OVER || __any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E))) {
+              if (!at_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
+              tc_fence_after();
+            }
+            if (__any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E)) {
+              const float mn = fmaxf(m2, top), corr = pg_ex2(m2 - mn);
               l *= corr;
               m2 = mn;
               if (t > k0) {
                 const float c2 = corr * exp2f((float)(E - En));
-                if (!at_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
-                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
                   uint32_t rg[16];
@@ -256,37 +289,29 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
                   for (int k = 0; k < 16; ++k) rg[k] = __float_as_uint(__uint_as_float(rg[k]) * c2);
                   tmem_st_32x16(tO + c * 16, rg);
                 }
-                tmem_st_wait();
               }
               E = En;
             }
             const float de[2] = {fmaxf((float)(e0 - En), -60.f), fmaxf((float)(e1 - En), -60.f)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float bias = TL_OFF + de[h] - m2;
-              float ls[4] = {0.f, 0.f, 0.f, 0.f};
+              const float2 ff = make_float2(f[h], f[h]), bias = make_float2(TL_OFF + de[h] - m2, TL_OFF + de[h] - m2);
+              float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                uint32_t rg[32], pk[16];
-                tmem_ld_32x32(tS + h * 64 + c * 32, rg);
-                tmem_ld_wait();
-                float e[32];
+                uint32_t pk[16];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) e[k] = pg_ex2(fmaf(__uint_as_float(rg[k]), f[h], bias));
-                if (mask) {
-#pragma unroll
-                  for (int k = 0; k < 32; ++k) {
-                    const int j = h * 64 + c * 32 + k;
-                    e[k] = j >= h_lo[h] && j <= h_hi[h] ? e[k] : 0.f;
-                  }
+                for (int k = 0; k < 16; ++k) {
+                  const int j = h * 64 + c * 32 + 2 * k;
+                  float2 e = tl_fma2(make_float2(x[j], x[j + 1]), ff, bias);
+                  e.x = pg_ex2(e.x);
+                  e.y = pg_ex2(e.y);
+                  ls[k & 1] = tl_add2(ls[k & 1], e);
+                  pk[k] = Cvt<__half>::pack2(e.x, e.y);
                 }
-#pragma unroll
-                for (int k = 0; k < 32; ++k) ls[k & 3] += e[k];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) pk[k] = Cvt<__half>::pack2(e[2 * k], e[2 * k + 1]);
-                tmem_st_32x16(tS + (2 * h + c) * 16, pk);
+                tmem_st_32x16(tP + (2 * h + c) * 16, pk);
               }
-              l = fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), exp2f(-de[h]), l);
+              l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), exp2f(-de[h]), l);
             }
             tmem_st_wait();
             tc_fence_before();
@@ -331,6 +356,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         w.next(p, G, cum, item.n, k1 - k0);
       }
     } else if (warp < 12) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_E));
       // ------------------------------------------------------------------------------------------ pages to float16
       const int tid = threadIdx.x - 256;
       constexpr int NK = HD / 16;                              // chunks of 16 codes a thread has of a tile's keys, and of its values
@@ -341,13 +367,18 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         const TlItem item = tl_item(p, w.s, G, w.qt);
         const int k0 = w.k, k1 = min(item.n, k0 + w.end - w.f), last = (w.s.start + w.s.n - 1) / PG;
         uint4 rk[NK], rv[NK];
-        int id[2];
-        auto fetch = [&](int t) {
+        int id[2], after[2];                                   // pages of the tile whose codes are on their way, and of the one behind it
+        float sc = 0.f;
+        auto look = [&](int t) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int pg = 2 * (item.lo + t) + h;
-            id[h] = pg <= last ? pg_page(a, w.b, pg) : -1;
+            after[h] = t < k1 && pg <= last ? pg_page(a, w.b, pg) : -1;
           }
+        };
+        auto fetch = [&](int t) {                              // codes of tile t, numbers of the pages of tile t + 1
+          id[0] = after[0];
+          id[1] = after[1];
           // chunk c of a page (HD * 64 codes): half h of the tile, in the order of memory
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
@@ -356,7 +387,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             rk[c] = id[h] < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(a.k + at)[ch];
             rv[c] = id[h] < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(a.v + at)[ch];
           }
+          if (tid < 4) {
+            const int page = tid & 1 ? id[1] : id[0];
+            sc = page >= 0 ? (tid < 2 ? a.ks : a.vs)[(long long)page * a.KV + w.g] : tid < 2 ? -1.f : PG_LEAST;
+          }
+          look(t + 1);
         };
+        look(k0);
         fetch(k0);
         for (int t = k0; t < k1; ++t, ++kv_it) {
           const int st = kv_it % L::STAGES;
@@ -383,12 +420,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             *reinterpret_cast<uint4*>(vp + sw128_off(vd, vt)) = make_uint4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<uint4*>(vp + sw128_off(vd, vt + 8)) = make_uint4(x[4], x[5], x[6], x[7]);
           }
-          if (tid == 0) {
-            float4 sc = make_float4(-1.f, -1.f, PG_LEAST, PG_LEAST);
-            if (id[0] >= 0) { sc.x = a.ks[(long long)id[0] * a.KV + w.g]; sc.z = a.vs[(long long)id[0] * a.KV + w.g]; }
-            if (id[1] >= 0) { sc.y = a.ks[(long long)id[1] * a.KV + w.g]; sc.w = a.vs[(long long)id[1] * a.KV + w.g]; }
-            scales[st] = sc;
-          }
+          if (tid < 4) reinterpret_cast<float*>(&scales[st])[tid] = sc;
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&kv_full[st]);
@@ -398,6 +430,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         w.next(p, G, cum, item.n, k1 - k0);
       }
     } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_I));
+      if (warp == 12) {
       // ------------------------------------------------------------------------------------------ MMAs
       const uint32_t on = elect_one();
       const uint32_t id_s = make_idesc_f16(0, 0, 0, 128, TL_KEYS), id_o = make_idesc_f16(0, 0, 0, 128, HD);
@@ -424,6 +458,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         }
         for (int t = k0; t < k1; ++t, ++kv_it) {
           if (t + 1 < k1) full(kv_it + 1);
+          if constexpr (!L::OVER) {
+            for (int wg = 0; wg < groups; ++wg) {
+              wait_or_report(&s_free[wg], it[wg] & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
+              tc_fence_after();
+              if (t + 1 < k1) scores(wg, kv_it + 1);
+            }
+          }
           const uint32_t sv = smem_u32(sKV + (kv_it % L::STAGES) * L::STAGE + L::K);
           for (int wg = 0; wg < groups; ++wg) {
             wait_or_report(&p_ready[wg], it[wg] & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
@@ -431,16 +472,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < TL_KEYS / 16; ++kk)
-              umma_f16_ts_on(on, tmem + 256 + wg * HD, tmem + wg * 128 + kk * 8, make_smem_desc_sw128(sv + (kk >> 2) * (HD * 128) + (kk & 3) * 32, 16, 1024), id_o,
-                             t > k0 || kk > 0 ? 1u : 0u);
+              umma_f16_ts_on(on, tmem + L::O0 + wg * HD, tmem + L::P0 + wg * L::P_STEP + kk * 8,
+                             make_smem_desc_sw128(sv + (kk >> 2) * (HD * 128) + (kk & 3) * 32, 16, 1024), id_o, t > k0 || kk > 0 ? 1u : 0u);
             umma_commit_on(on, &o_full[wg]);
             if (wg == groups - 1) umma_commit_on(on, &kv_empty[kv_it % L::STAGES]);
-            if (t + 1 < k1) scores(wg, kv_it + 1);
+            if (L::OVER && t + 1 < k1) scores(wg, kv_it + 1);
           }
         }
         w.next(p, G, cum, item.n, k1 - k0);
       }
       __syncwarp();
+      }
     }
   }
   __syncthreads();
@@ -497,7 +539,7 @@ template <typename T, int HD>
 static int tl_go(const PgAttn& p, cudaStream_t st) {
   using L = Tl<HD>;
   // at least 120 KB, so that one block takes an SM with its tensor memory
-  const size_t smem = std::max<size_t>(120 * 1024, 1024 + 2 * L::Q + L::STAGES * (L::STAGE + 32) + 64 + 16 + (size_t)(p.a.B + 1) * 4);
+  const size_t smem = std::max<size_t>(120 * 1024, 1024 + 2 * L::Q + L::STAGES * (L::STAGE + 32) + 80 + 16 + (size_t)(p.a.B + 1) * 4);
   const int blocks = pg_sms();
   GB_PDL_LAUNCH_SMEM((paged_tile_kernel<T, HD>), dim3(blocks), dim3(TL_THREADS), smem, st, p);
   const int rc = gb_launch_rc();
