@@ -53,7 +53,12 @@ __device__ __forceinline__ float2 tl_add2(float2 a, float2 b) {
   return d;
 }
 
-struct TlItem { int lo, n; };                                 // first key tile, number of them
+constexpr int TL_AHEAD = 1;
+struct TlItem {
+  int lo, n;                                                  // first key tile, number of them
+  // an item has n + TL_AHEAD places; those of a run that are its places k0 ... k1 - 1 are these key tiles
+  __device__ __forceinline__ int tile(int k) const { return max(0, k - TL_AHEAD); }
+};
 __device__ __forceinline__ TlItem tl_item(const PgAttn& p, const PgSeq& s, int G, int qt) {
   const int r1 = min(s.n * G, (qt + 1) * TL_ROWS) - 1;
   const int p0 = s.start + qt * TL_ROWS / G, p1 = s.start + r1 / G;
@@ -63,17 +68,23 @@ __device__ __forceinline__ TlItem tl_item(const PgAttn& p, const PgSeq& s, int G
 
 // A block's walk over its run: places f ... end, one piece of an item after the other.
 struct TlWalk {
-  int f, end, b, g, qt, k;                                    // k: key tiles of the item that come before place f
+  int f, end, b, g, qt, k;                                    // k: places of the item that come before place f
   PgSeq s;
   int tiles;
   __device__ __forceinline__ void load(const PgAttn& p, int G) {
     s = pg_seq(p.a, b);
     tiles = (s.n * G + TL_ROWS - 1) / TL_ROWS;
   }
-  __device__ __forceinline__ void next(const PgAttn& p, int G, const int* cum, int n, int taken) {
+  // the run's part of this item: key tiles k0 ... k1 - 1
+  __device__ __forceinline__ void part(const TlItem& item, int& k0, int& k1) const {
+    k0 = item.tile(k);
+    k1 = item.tile(min(item.n + TL_AHEAD, k + end - f));
+  }
+  __device__ __forceinline__ void next(const PgAttn& p, int G, const int* cum, const TlItem& item) {
+    const int taken = min(item.n + TL_AHEAD - k, end - f);
     f += taken;
     k += taken;
-    if (k < n || f >= end) return;
+    if (k < item.n + TL_AHEAD || f >= end) return;
     k = 0;
     if (++qt < tiles) return;
     qt = 0;
@@ -91,17 +102,20 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sKV = smem + 2 * L::Q;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + L::STAGES * L::STAGE);
-  uint64_t *kv_full = bars, *kv_empty = bars + L::STAGES, *s_full = bars + 2 * L::STAGES, *p_ready = s_full + 2, *o_full = s_full + 4, *q_full = s_full + 6, *s_free = s_full + 8;
-  float4* scales = reinterpret_cast<float4*>(bars + 2 * L::STAGES + 10);      // of a stage: key scales of its two pages, value scales; a negative key scale: no page
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scales + L::STAGES);
+  uint64_t *k_full = bars, *k_empty = k_full + L::STAGES, *v_full = k_empty + L::STAGES, *v_empty = v_full + L::STAGES;
+  uint64_t *s_full = v_empty + L::STAGES, *p_ready = s_full + 2, *o_full = s_full + 4, *q_full = s_full + 6, *s_free = s_full + 8, *turn = s_full + 10;
+  uint64_t* sc_full = turn + 2;                                               // 4: of a key tile's scales, which outlive its stage
+  float4* scales = reinterpret_cast<float4*>(sc_full + 4);      // of a stage: key scales of its two pages, value scales; a negative key scale: no page
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scales + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* cum = reinterpret_cast<int*>(tmem_slot + 2);                           // key tiles (of one head) of the sequences before
   const gb_paged& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.H / a.KV;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L::STAGES; ++s) { mbar_init(&kv_full[s], 4); mbar_init(&kv_empty[s], 1); }
-    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); }
+    for (int s = 0; s < L::STAGES; ++s) { mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1); }
+    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); mbar_init(&turn[w], 4); }
+    for (int s = 0; s < 4; ++s) mbar_init(&sc_full[s], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -112,7 +126,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
     const PgSeq s = pg_seq(a, b);
     const int tiles = (s.n * G + TL_ROWS - 1) / TL_ROWS;
     int n = 0;
-    for (int qt = lane; qt < tiles; qt += 32) n += tl_item(p, s, G, qt).n;
+    for (int qt = lane; qt < tiles; qt += 32) n += tl_item(p, s, G, qt).n + TL_AHEAD;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     if (lane == 0) cum[b + 1] = n;
@@ -156,7 +170,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
     start.qt = 0;
     start.k = 0;
     for (int q0 = 0; q0 < start.tiles; q0 += 32) {            // the item that holds place f: a warp looks through 32 at a time
-      const int n = q0 + lane < start.tiles ? tl_item(p, start.s, G, q0 + lane).n : 0;
+      const int n = q0 + lane < start.tiles ? tl_item(p, start.s, G, q0 + lane).n + TL_AHEAD : 0;
       int v = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -180,13 +194,16 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       const uint32_t row = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tS = tmem + wg * 128 + row, tP = tmem + L::P0 + wg * L::P_STEP + row, tO = tmem + L::O0 + wg * HD + row;
       uint8_t* q_at = sQ + wg * L::Q;
-      uint32_t kv_it = 0, it = 0;                              // key tiles so far; those of this warpgroup
+      uint32_t kv_it = 0, it = 0, turns = 0;                   // key tiles so far; those of this warpgroup; its turns at the exponentials
       bool ok = true;
       TlWalk w = start;
       while (w.f < w.end && ok) {
         const TlItem item = tl_item(p, w.s, G, w.qt);
-        const int k0 = w.k, k1 = min(item.n, k0 + w.end - w.f), rows = w.s.n * G, first = w.qt * TL_ROWS + wg * 128;
-        if (first < rows) {
+        const int rows = w.s.n * G, first = w.qt * TL_ROWS + wg * 128;
+        int k0, k1;
+        w.part(item, k0, k1);
+        if (first < rows && k0 < k1) {
+          const bool both = w.qt * TL_ROWS + 128 < rows;       // the other warpgroup has rows too
           const int rr = first + r, i = rr / G, pos = w.s.start + i;
           const bool row_ok = rr < rows;
           const int pos_a = w.s.start + first / G, pos_z = w.s.start + (min(rows, first + 128) - 1) / G;
@@ -227,11 +244,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           float m2 = -1e30f, l = 0.f;
           int E = -1000;
           for (int t = k0; t < k1; ++t, ++it, ++kv_it) {
-            const int st = kv_it % L::STAGES;
             if (!at_wait(&s_full[wg], it & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag) ||
-                !at_wait(&kv_full[st], (kv_it / L::STAGES) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag)) { ok = false; break; }
+                !at_wait(&sc_full[kv_it & 3], (kv_it >> 2) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag)) { ok = false; break; }
             tc_fence_after();
-            const float4 sc = scales[st];
+            const float4 sc = scales[kv_it & 3];
             float x[128];
             {
               uint32_t(*rg)[32] = reinterpret_cast<uint32_t(*)[32]>(x);
@@ -292,6 +308,11 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
               }
               E = En;
             }
+            // exponentials in turn: while one warpgroup has the unit that makes them, the other loads and looks for maxima
+            if (both) {
+              if (!at_wait(&turn[wg], (turns & 1u) ^ (wg == 0 ? 1u : 0u), a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
+              ++turns;
+            }
             const float de[2] = {fmaxf((float)(e0 - En), -60.f), fmaxf((float)(e1 - En), -60.f)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -313,6 +334,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
               }
               l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), exp2f(-de[h]), l);
             }
+            if (both && lane == 0) mbar_arrive(&turn[wg ^ 1]);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -322,7 +344,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           if (!at_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const bool whole = k0 == 0 && k1 == item.n;
-          const int f0 = w.f - k0, slot = 2 * blockIdx.x + (f0 > start.f ? 1 : 0);
+          const int f0 = w.f - w.k + TL_AHEAD, slot = 2 * blockIdx.x + (f0 > start.f ? 1 : 0);
           float* rec = records + (size_t)slot * L::REC;
           const float fac = l == 0.f ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23) / l;
           T* dst = reinterpret_cast<T*>(p.out) + (long long)(w.s.first + i) * p.ld_o + (long long)(w.g * G + rr - i * G) * HD;
@@ -353,7 +375,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         } else {
           kv_it += k1 - k0;
         }
-        w.next(p, G, cum, item.n, k1 - k0);
+        w.next(p, G, cum, item);
       }
     } else if (warp < 12) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_E));
@@ -365,44 +387,57 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       TlWalk w = start;
       while (w.f < w.end && ok) {
         const TlItem item = tl_item(p, w.s, G, w.qt);
-        const int k0 = w.k, k1 = min(item.n, k0 + w.end - w.f), last = (w.s.start + w.s.n - 1) / PG;
+        const int last = (w.s.start + w.s.n - 1) / PG;
+        int k0, k1;
+        w.part(item, k0, k1);
         uint4 rk[NK], rv[NK];
-        int id[2], after[2];                                   // pages of the tile whose codes are on their way, and of the one behind it
+        int id[2], after[2];                                   // pages of the tile whose codes are on their way; what the table has for the one behind it
         float sc = 0.f;
-        auto look = [&](int t) {
+        auto look = [&](int t) {                               // nothing waits for the answer here
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int pg = 2 * (item.lo + t) + h;
-            after[h] = t < k1 && pg <= last ? pg_page(a, w.b, pg) : -1;
+            after[h] = t < k1 && pg <= last ? a.table[(long long)w.b * a.W + pg] : -2;
           }
         };
-        auto fetch = [&](int t) {                              // codes of tile t, numbers of the pages of tile t + 1
-          id[0] = after[0];
-          id[1] = after[1];
-          // chunk c of a page (HD * 64 codes): half h of the tile, in the order of memory
+        // codes of a tile's keys or values, chunk c of a page (HD * 64 codes) in the order of memory
+        auto fetch = [&](uint4 (&r)[NK], const signed char* from) {
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
             const int h = c / (NK / 2), ch = (c % (NK / 2)) * 128 + tid;
             const long long at = ((long long)max(id[h], 0) * a.KV + w.g) * (PG * HD);
-            rk[c] = id[h] < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(a.k + at)[ch];
-            rv[c] = id[h] < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(a.v + at)[ch];
+            r[c] = id[h] < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(from + at)[ch];
           }
+        };
+        auto fetch_keys = [&](int t) {                         // and the scales of tile t, the pages' numbers of tile t + 1
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            id[h] = after[h];
+            if ((unsigned)id[h] >= (unsigned)a.pages) {
+              if (id[h] != -2 || 2 * (item.lo + t) + h <= last) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
+              id[h] = -1;
+            }
+          }
+          fetch(rk, a.k);
           if (tid < 4) {
             const int page = tid & 1 ? id[1] : id[0];
             sc = page >= 0 ? (tid < 2 ? a.ks : a.vs)[(long long)page * a.KV + w.g] : tid < 2 ? -1.f : PG_LEAST;
           }
           look(t + 1);
         };
-        look(k0);
-        fetch(k0);
+        if (k0 < k1) {
+          look(k0);
+          fetch_keys(k0);
+          fetch(rv, a.v);
+        }
         for (int t = k0; t < k1; ++t, ++kv_it) {
           const int st = kv_it % L::STAGES;
-          if (!at_wait(&kv_empty[st], ((kv_it / L::STAGES) & 1u) ^ 1u, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
+          const uint32_t free = ((kv_it / L::STAGES) & 1u) ^ 1u;
           uint8_t *sk = sKV + st * L::STAGE, *sv = sk + L::K;
+          if (!at_wait(&k_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
-            const int h = c / (NK / 2), ch = (c % (NK / 2)) * 128 + tid;
-            const int key = h * 64 + ch / (HD / 16), d = (ch % (HD / 16)) * 16;               // 16 dimensions of a key
+            const int ch = (c % (NK / 2)) * 128 + tid, key = c / (NK / 2) * 64 + ch / (HD / 16), d = (ch % (HD / 16)) * 16;      // 16 dimensions of a key
             uint32_t x[8];
             pg_halves(rk[c].x, x[0], x[1]);
             pg_halves(rk[c].y, x[2], x[3]);
@@ -411,23 +446,33 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             uint8_t* kp = sk + (d >> 6) * (128 * 128);
             *reinterpret_cast<uint4*>(kp + sw128_off(key, d & 63)) = make_uint4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<uint4*>(kp + sw128_off(key, (d & 63) + 8)) = make_uint4(x[4], x[5], x[6], x[7]);
-            const int vd = ch >> 2, vt = (ch & 3) * 16;                                       // 16 tokens of a dimension
+          }
+          if (tid < 4) reinterpret_cast<float*>(&scales[kv_it & 3])[tid] = sc;
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&k_full[st]);
+          if (tid == 0) mbar_arrive(&sc_full[kv_it & 3]);
+          if (t + 1 < k1) fetch_keys(t + 1);
+          if (!at_wait(&v_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
+#pragma unroll
+          for (int c = 0; c < NK; ++c) {
+            const int ch = (c % (NK / 2)) * 128 + tid, vd = ch >> 2, vt = (ch & 3) * 16;                                          // 16 tokens of a dimension
+            uint32_t x[8];
             pg_halves(rv[c].x, x[0], x[1]);
             pg_halves(rv[c].y, x[2], x[3]);
             pg_halves(rv[c].z, x[4], x[5]);
             pg_halves(rv[c].w, x[6], x[7]);
-            uint8_t* vp = sv + h * (HD * 128);
+            uint8_t* vp = sv + c / (NK / 2) * (HD * 128);
             *reinterpret_cast<uint4*>(vp + sw128_off(vd, vt)) = make_uint4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<uint4*>(vp + sw128_off(vd, vt + 8)) = make_uint4(x[4], x[5], x[6], x[7]);
           }
-          if (tid < 4) reinterpret_cast<float*>(&scales[st])[tid] = sc;
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&kv_full[st]);
-          if (t + 1 < k1) fetch(t + 1);
+          if (lane == 0) mbar_arrive(&v_full[st]);
+          if (t + 1 < k1) fetch(rv, a.v);
         }
         if (!ok) break;
-        w.next(p, G, cum, item.n, k1 - k0);
+        w.next(p, G, cum, item);
       }
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_I));
@@ -437,34 +482,39 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       const uint32_t id_s = make_idesc_f16(0, 0, 0, 128, TL_KEYS), id_o = make_idesc_f16(0, 0, 0, 128, HD);
       uint32_t kv_it = 0, q_it[2] = {0, 0}, it[2] = {0, 0};
       TlWalk w = start;
-      auto scores = [&](int wg, uint32_t at) {
-        mma_kmajor_kmajor<HD>(on, tmem + wg * 128, smem_u32(sQ + wg * L::Q), smem_u32(sKV + (at % L::STAGES) * L::STAGE), id_s, false);
-        umma_commit_on(on, &s_full[wg]);
-      };
-      auto full = [&](uint32_t at) {
-        wait_or_report(&kv_full[at % L::STAGES], (at / L::STAGES) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
+      auto full = [&](uint64_t* bar, uint32_t at) {
+        wait_or_report(&bar[at % L::STAGES], (at / L::STAGES) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
         tc_fence_after();
       };
       while (w.f < w.end) {
         const TlItem item = tl_item(p, w.s, G, w.qt);
-        const int k0 = w.k, k1 = min(item.n, k0 + w.end - w.f);
+        int k0, k1;
+        w.part(item, k0, k1);
         const int groups = w.qt * TL_ROWS + 128 < w.s.n * G ? 2 : 1;
-        full(kv_it);
-        for (int wg = 0; wg < groups; ++wg) {
-          wait_or_report(&q_full[wg], q_it[wg] & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
-          ++q_it[wg];
-          tc_fence_after();
-          scores(wg, kv_it);
+        auto scores = [&](int wg, uint32_t at) {
+          mma_kmajor_kmajor<HD>(on, tmem + wg * 128, smem_u32(sQ + wg * L::Q), smem_u32(sKV + (at % L::STAGES) * L::STAGE), id_s, false);
+          umma_commit_on(on, &s_full[wg]);
+          if (wg == groups - 1) umma_commit_on(on, &k_empty[at % L::STAGES]);
+        };
+        if (k0 < k1) {
+          full(k_full, kv_it);
+          for (int wg = 0; wg < groups; ++wg) {
+            wait_or_report(&q_full[wg], q_it[wg] & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
+            ++q_it[wg];
+            tc_fence_after();
+            scores(wg, kv_it);
+          }
         }
         for (int t = k0; t < k1; ++t, ++kv_it) {
-          if (t + 1 < k1) full(kv_it + 1);
-          if constexpr (!L::OVER) {
+          if (!L::OVER) {
+            if (t + 1 < k1) full(k_full, kv_it + 1);
             for (int wg = 0; wg < groups; ++wg) {
               wait_or_report(&s_free[wg], it[wg] & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
               tc_fence_after();
               if (t + 1 < k1) scores(wg, kv_it + 1);
             }
           }
+          full(v_full, kv_it);
           const uint32_t sv = smem_u32(sKV + (kv_it % L::STAGES) * L::STAGE + L::K);
           for (int wg = 0; wg < groups; ++wg) {
             wait_or_report(&p_ready[wg], it[wg] & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
@@ -475,11 +525,14 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
               umma_f16_ts_on(on, tmem + L::O0 + wg * HD, tmem + L::P0 + wg * L::P_STEP + kk * 8,
                              make_smem_desc_sw128(sv + (kk >> 2) * (HD * 128) + (kk & 3) * 32, 16, 1024), id_o, t > k0 || kk > 0 ? 1u : 0u);
             umma_commit_on(on, &o_full[wg]);
-            if (wg == groups - 1) umma_commit_on(on, &kv_empty[kv_it % L::STAGES]);
-            if (L::OVER && t + 1 < k1) scores(wg, kv_it + 1);
+            if (wg == groups - 1) umma_commit_on(on, &v_empty[kv_it % L::STAGES]);
+            if (L::OVER && t + 1 < k1) {
+              full(k_full, kv_it + 1);
+              scores(wg, kv_it + 1);
+            }
           }
         }
-        w.next(p, G, cum, item.n, k1 - k0);
+        w.next(p, G, cum, item);
       }
       __syncwarp();
       }
@@ -539,7 +592,7 @@ template <typename T, int HD>
 static int tl_go(const PgAttn& p, cudaStream_t st) {
   using L = Tl<HD>;
   // at least 120 KB, so that one block takes an SM with its tensor memory
-  const size_t smem = std::max<size_t>(120 * 1024, 1024 + 2 * L::Q + L::STAGES * (L::STAGE + 32) + 80 + 16 + (size_t)(p.a.B + 1) * 4);
+  const size_t smem = std::max<size_t>(120 * 1024, 1024 + 2 * L::Q + L::STAGES * (L::STAGE + 32) + 16 * 8 + 64 + 16 + (size_t)(p.a.B + 1) * 4);
   const int blocks = pg_sms();
   GB_PDL_LAUNCH_SMEM((paged_tile_kernel<T, HD>), dim3(blocks), dim3(TL_THREADS), smem, st, p);
   const int rc = gb_launch_rc();
