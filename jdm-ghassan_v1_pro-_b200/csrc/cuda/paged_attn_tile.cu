@@ -30,12 +30,17 @@ struct Tl {
   static constexpr bool OVER = HD == 128;
   static constexpr int P0 = OVER ? 0 : 256, P_STEP = OVER ? 128 : 64, O0 = OVER ? 256 : 384;
   // registers a thread: soft-max, expanding, issuing; launched with 128, so 2 x 128 x S + 128 x (E + I) is at most 65536
-  static constexpr int REGS_S = HD == 128 ? 184 : 192, REGS_E = HD == 128 ? 104 : 88, REGS_I = 40;
+  static constexpr int REGS_S = 184, REGS_E = HD == 128 ? 104 : 88, REGS_I = HD == 128 ? 40 : 56;
   static constexpr int REC = TL_ROWS * (HD + 2);              // floats of a record: [HD / 4][256] four results, then [256] pairs (maximum, sum)
 };
 
 // What a record is of: places of its item, and which it is.  f1 == 0: nothing.
 struct TlDesc { int f0, f1, b, g, qt, quota, pad0, pad1; };
+
+// Bounded waits: false once the block has given up.  The first polls are all that a phase takes that is over already.  (The rest is no call: there are 128 scores in registers.)
+__device__ __forceinline__ bool tl_wait(uint64_t* bar, uint32_t parity, int* status, int code, volatile int* abort_flag) {
+  return mbar_try_wait_some(bar, parity) || at_wait(bar, parity, status, code, abort_flag);
+}
 
 // Two fp32 operations an instruction.
 __device__ __forceinline__ float2 tl_fma2(float2 a, float2 b, float2 c) {
@@ -104,8 +109,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + L::STAGES * L::STAGE);
   uint64_t *k_full = bars, *k_empty = k_full + L::STAGES, *v_full = k_empty + L::STAGES, *v_empty = v_full + L::STAGES;
   uint64_t *s_full = v_empty + L::STAGES, *p_ready = s_full + 2, *o_full = s_full + 4, *q_full = s_full + 6, *s_free = s_full + 8, *turn = s_full + 10;
-  uint64_t* sc_full = turn + 2;                                               // 4: of a key tile's scales, which outlive its stage
-  float4* scales = reinterpret_cast<float4*>(sc_full + 4);      // of a stage: key scales of its two pages, value scales; a negative key scale: no page
+  float4* scales = reinterpret_cast<float4*>(turn + 2);                       // of four key tiles (they outlive a stage): key scales of the two pages, value scales; a negative
+                                                                              // key scale: no page
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scales + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* cum = reinterpret_cast<int*>(tmem_slot + 2);                           // key tiles (of one head) of the sequences before
@@ -114,8 +119,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) { mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1); }
-    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); mbar_init(&turn[w], 4); }
-    for (int s = 0; s < 4; ++s) mbar_init(&sc_full[s], 1);
+    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 2); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); mbar_init(&turn[w], 4); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -244,8 +248,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           float m2 = -1e30f, l = 0.f;
           int E = -1000;
           for (int t = k0; t < k1; ++t, ++it, ++kv_it) {
-            if (!at_wait(&s_full[wg], it & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag) ||
-                !at_wait(&sc_full[kv_it & 3], (kv_it >> 2) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag)) { ok = false; break; }
+            if (!tl_wait(&s_full[wg], it & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
             tc_fence_after();
             const float4 sc = scales[kv_it & 3];
             float x[128];
@@ -262,10 +265,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             }
             const int base = (item.lo + t) * TL_KEYS;
             if (base + TL_KEYS - 1 > pos_a || (p.window > 0 && pos_z - p.window + 1 > base) || sc.x < 0.f || sc.y < 0.f) {
+              // a bit a column, so that a column costs a test and a choice: three comparisons each were a third of the loop's code, and its fetching showed
               const int hi = pos - base, lo = p.window > 0 ? pos - p.window + 1 - base : 0;
 #pragma unroll
-              for (int k = 0; k < 128; ++k)
-                if (k > hi || k < lo || (k < 64 ? sc.x : sc.y) < 0.f) x[k] = -INFINITY;
+              for (int w = 0; w < 4; ++w) {
+                const int h = hi - 32 * w, l0 = lo - 32 * w;              // columns l0 ... h of this word
+                uint32_t see = (h >= 31 ? 0xffffffffu : h < 0 ? 0u : (2u << h) - 1u) & (l0 <= 0 ? 0xffffffffu : l0 > 31 ? 0u : 0xffffffffu << l0);
+                if ((w < 2 ? sc.x : sc.y) < 0.f) see = 0u;
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  if (!(see & (1u << k))) x[32 * w + k] = -INFINITY;
+              }
             }
             // a factor that is too small for fp32 must not make nothing of a hidden score
             float f[2] = {qs * fabsf(sc.x), qs * fabsf(sc.y)};
@@ -286,11 +296,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             const float top = fmaxf(mt[0], mt[1]);
             const int e0 = (int)(__float_as_uint(sc.z) >> 23) - 127, e1 = (int)(__float_as_uint(sc.w) >> 23) - 127, En = max(E, max(e0, e1));
             // the last second product is done: its weights' places are free, its sums can be rescaled
-            if (t > k0 && (!L::OVER || __any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E))) {
-              if (!at_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
+            const bool grow = __any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E);
+            if (t > k0 && (!L::OVER || grow)) {
+              if (!tl_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
               tc_fence_after();
             }
-            if (__any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E)) {
+            if (grow) {
               const float mn = fmaxf(m2, top), corr = pg_ex2(m2 - mn);
               l *= corr;
               m2 = mn;
@@ -310,7 +321,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             }
             // exponentials in turn: while one warpgroup has the unit that makes them, the other loads and looks for maxima
             if (both) {
-              if (!at_wait(&turn[wg], (turns & 1u) ^ (wg == 0 ? 1u : 0u), a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
+              if (!tl_wait(&turn[wg], (turns & 1u) ^ (wg == 0 ? 1u : 0u), a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
               ++turns;
             }
             const float de[2] = {fmaxf((float)(e0 - En), -60.f), fmaxf((float)(e1 - En), -60.f)};
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             if (lane == 0) mbar_arrive(&p_ready[wg]);
           }
           if (!ok) break;
-          if (!at_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
+          if (!tl_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const bool whole = k0 == 0 && k1 == item.n;
           const int f0 = w.f - w.k + TL_AHEAD, slot = 2 * blockIdx.x + (f0 > start.f ? 1 : 0);
@@ -434,7 +445,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           const int st = kv_it % L::STAGES;
           const uint32_t free = ((kv_it / L::STAGES) & 1u) ^ 1u;
           uint8_t *sk = sKV + st * L::STAGE, *sv = sk + L::K;
-          if (!at_wait(&k_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
+          if (!tl_wait(&k_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
             const int ch = (c % (NK / 2)) * 128 + tid, key = c / (NK / 2) * 64 + ch / (HD / 16), d = (ch % (HD / 16)) * 16;      // 16 dimensions of a key
@@ -451,9 +462,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&k_full[st]);
-          if (tid == 0) mbar_arrive(&sc_full[kv_it & 3]);
           if (t + 1 < k1) fetch_keys(t + 1);
-          if (!at_wait(&v_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
+          if (!tl_wait(&v_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
             const int ch = (c % (NK / 2)) * 128 + tid, vd = ch >> 2, vt = (ch & 3) * 16;                                          // 16 tokens of a dimension
@@ -493,6 +503,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         const int groups = w.qt * TL_ROWS + 128 < w.s.n * G ? 2 : 1;
         auto scores = [&](int wg, uint32_t at) {
           mma_kmajor_kmajor<HD>(on, tmem + wg * 128, smem_u32(sQ + wg * L::Q), smem_u32(sKV + (at % L::STAGES) * L::STAGE), id_s, false);
+          if (on) mbar_arrive(&s_full[wg]);                    // hands on what k_full brought: the scales, which no MMA touches
           umma_commit_on(on, &s_full[wg]);
           if (wg == groups - 1) umma_commit_on(on, &k_empty[at % L::STAGES]);
         };
