@@ -36,7 +36,7 @@ def _parser() -> argparse.ArgumentParser:
     ap.add_argument("command", choices=["chat", "generate", "info", "quantize", "bench", "tokenize", "export", "eval",
                                         "perplexity", "devices", "logits"])
     for name in ("model", "prompt", "out", "profile", "tokenizer", "text", "checkpoint", "suite", "shards", "prefix", "system",
-                 "persona", "retrieve-index", "categories", "format", "compat", "ids"):
+                 "persona", "retrieve-index", "categories", "format", "compat", "ids", "kv-cache"):
         ap.add_argument("--" + name)
     for name, typ in (("temp", float), ("top-k", int), ("top-p", float), ("min-p", float), ("repeat", float),
                       ("no-repeat-ngram", int), ("max-tokens", int), ("seed", int), ("tokens", int), ("prompt-tokens", int),
@@ -117,7 +117,10 @@ def _load(a, batch=1, ctx=0):
         if a.yarn_mscale is not None:
             m.cfg.rope_yarn_mscale = float(a.yarn_mscale)
         m.cfg.validate()
-    eng = IO.build_engine(m, batch=batch, max_len=ctx or min(2048, m.cfg.max_seq_len), fmt=a.format or "auto")
+    try:
+        eng = IO.build_engine(m, batch=batch, max_len=ctx or min(2048, m.cfg.max_seq_len), fmt=a.format or "auto", kv_cache=a.kv_cache or "16bit")
+    except ValueError as e:
+        raise SystemExit(str(e)) if a.kv_cache else e
     return m, Generator(eng, m.tokenizer)
 
 

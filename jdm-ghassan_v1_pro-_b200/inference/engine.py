@@ -8,7 +8,8 @@ candidates back for every token.  Here:
 * weights stay in their storage format (fp16 / bf16 / ggml Q8_0 / Q4_0 / internal Q8_0(64) / Q4_1) and are
   expanded inside the GEMV kernels (``csrc/cuda/decode.cu``); the prompt pass uses 16-bit copies with the GEMM;
 * the KV cache is 16-bit ``[batch, capacity, kv_dim]`` per layer with the reference's slot rule: the first 8 tokens
-  are pinned, later slots form a ring (inference/kv_cache.h:11-106);
+  are pinned, later slots form a ring (inference/kv_cache.h:11-106); or, with ``kv_cache="q8"``, pages of 8-bit codes (``ops/paged.py``), half the
+  memory, for sequences up to ``max_len`` tokens, whose prompts of any length go through the batched pass portion by portion;
 * positions, cache lengths, router choices, sampled tokens, stop flags and the token transcript all live on the
   device, so a decode step has no host dependency and is captured once;
 * the sampler is a device kernel fed with uniform numbers drawn from the same generator a host sampler would use.
@@ -27,6 +28,7 @@ from ..models.config import ModelConfig
 from ..models.cuda_model import CudaModel
 from ..ops import decode as D
 from ..ops import kernels as K
+from ..ops import paged as P
 from ..utils import canary as CA
 from .token_loop import SamplingParams, TokenLoop  # noqa: F401  (SamplingParams is re-exported)
 
@@ -71,15 +73,20 @@ class InferenceEngine(TokenLoop):
     def __init__(self, cfg: ModelConfig, named: Dict[str, np.ndarray], fmt: str = "f16", batch: int = 1,
                  max_len: int = 2048, prefill_chunk: int = 1024, moe_bias: Optional[Sequence] = None, device=None,
                  compute_dtype=torch.float16, keep_f16_embeddings: bool = True, raw=None, raw_types=None,
-                 fused_step: bool = True, single_kernel: Optional[bool] = None, gemm_min_batch: Optional[int] = None):
+                 fused_step: bool = True, single_kernel: Optional[bool] = None, gemm_min_batch: Optional[int] = None,
+                 kv_cache: str = "16bit"):
         """``named``: fp32 tensors by parameter name.  ``fmt``: decode weight format, or "auto" with ``raw`` (an object
         with ``tensor_raw(name)``, e.g. a GGUF file) and ``raw_types`` (name -> ggml type) to take the stored bytes.
         ``single_kernel``: run the token step of a batch of one as one cooperative kernel (``csrc/cuda/decode_mega.cu``)
         when the shapes allow it; None takes the default (on; ``GB200_DECODE_MEGA=0`` turns it off).  ``gemm_min_batch``: from this many
         sequences on, the token step runs its projections and experts as tensor-core GEMMs over 16-bit copies of the
         weights (the ones the prompt pass keeps) instead of per-sequence GEMV kernels over the stored bytes; None
-        takes ``GB200_DECODE_GEMM_MIN_BATCH`` (default 8), 0 turns it off."""
+        takes ``GB200_DECODE_GEMM_MIN_BATCH`` (default 8), 0 turns it off.  ``kv_cache``: "16bit" or "q8" (8-bit pages; sequences end at
+        ``max_len``, and the kernel chain takes the token step)."""
         cfg.validate()
+        if kv_cache not in ("16bit", "q8"):
+            raise ValueError("kv_cache is 16bit or q8, not %s" % kv_cache)
+        self.paged = kv_cache == "q8"
         if cfg.head_dim not in (32, 64, 128):
             raise ValueError("decode attention supports head_dim 32, 64 and 128")
         self.cfg, self.B, self.cap, self.pinned = cfg, batch, max_len, PINNED_TOKENS
@@ -149,14 +156,17 @@ class InferenceEngine(TokenLoop):
                 L.ws = K.MoeWorkspace(batch, d, cfg.num_experts, cfg.moe_top_k, cfg.moe_shared, self.dt, self.dev)
             else:
                 L.wg, L.wu, L.wd = q(r + "w_gate"), q(r + "w_up"), q(r + "w_down")
-            L.cK = CA.zeros(batch, max_len, kvd, **c16)
-            L.cV = CA.zeros(batch, max_len, kvd, **c16)
+            if self.paged:
+                L.pages = P.new_pages(batch * -(-max_len // P.PAGE), cfg.num_kv_heads, cfg.head_dim, self.dev)
+            else:
+                L.cK = CA.zeros(batch, max_len, kvd, **c16)
+                L.cV = CA.zeros(batch, max_len, kvd, **c16)
             self.layers.append(L)
         self.weight_bytes = sum(w.nbytes for L in self.layers for w in (L.wqkv, L.wo, L.wg, L.wu, L.wd)) + self.head.nbytes
         # ---- decode state and buffers (all static: one graph serves every step)
         B = batch
         self._init_loop(B, V, max_len)
-        self.slot_pos = CA.zeros(B, max_len, **i32)
+        self.slot_pos = None if self.paged else CA.zeros(B, max_len, **i32)
         self.x = [CA.zeros(B, d, **f32) for _ in range(2)]
         self.x_mid = CA.zeros(B, d, **f32)
         self.xb = CA.zeros(B, d, **c16)
@@ -178,9 +188,16 @@ class InferenceEngine(TokenLoop):
         self.mega: Optional[D.MegaArgs] = None
         if single_kernel is None:
             single_kernel = os.environ.get("GB200_DECODE_MEGA", "1") != "0"
-        if single_kernel and batch == 1:
+        if single_kernel and batch == 1 and not self.paged:
             self._build_mega()
         self.prefill_chunk = min(prefill_chunk, max_len)
+        if self.paged:
+            W, T, C = -(-max_len // P.PAGE), self.prefill_chunk, cfg
+            self.table = torch.arange(B * W, **i32).view(B, W)                     # one for all layers
+            self.prompt_first, self.prompt_count = torch.arange(0, B * T, T, **i32), torch.zeros(B, **i32)
+            need = [P.attn_scratch(B, W, C.num_kv_heads, C.head_dim, n, C.num_heads, C.sliding_window) for n in (1, T)]
+            self.kv_scratch = CA.empty(max(4, *need), **f32)
+        self._len, self._claimed = 0, False                                        # tokens of every sequence, as the host counts them (paged caches)
         self._prefill_model: Optional[CudaModel] = None
         self._prompt_seen = False
         self._prompt_graph: Optional[torch.cuda.CUDAGraph] = None
@@ -255,6 +272,50 @@ class InferenceEngine(TokenLoop):
         out["step"] = float(acc.sum())
         return out
 
+    # ------------------------------------------------------------------ paged caches
+    @property
+    def token_limit(self) -> Optional[int]:
+        """Most tokens a sequence may have, or None (the ring cache keeps the first and the most recent ones)."""
+        return self.cap if self.paged else None
+
+    def _claim(self, n: int):
+        """Counts ``n`` more tokens of every sequence; refuses what the pages cannot hold."""
+        if self.paged:
+            if self._len + n > self.cap:
+                raise ValueError("sequence would exceed the %d tokens this engine was sized for" % self.cap)
+            self._len += n
+
+    def check(self, what: str = "generation"):
+        """Raise if a kernel recorded a failure (waits for the device)."""
+        from ..ops import _lib
+        _lib.check_status(self.dev, what)
+
+    def reset(self, seed: int = 0):
+        super().reset(seed)
+        self._len = 0
+
+    def decode_steps(self, n: int, sp: SamplingParams, use_graph: bool = True):
+        if n > 0 and sp.device_ok():
+            self._claim(n)
+        self._claimed = True          # counted here: replays of the captured step do not pass through Python
+        try:
+            super().decode_steps(n, sp, use_graph)
+        finally:
+            self._claimed = False
+
+    def paged_step(self, L: _Layer, qkv, q, att):
+        """One token's rows of every sequence through a layer's pages: ``qkv`` to rotated ``q``, keys and values stored, attention into ``att``."""
+        cfg = self.cfg
+        P.append(L.pages, qkv, self.table, self.pos, 1, self.cos_sin, cfg.num_heads, q_out=q, qw=L.qn, kw=L.kn, eps=cfg.rms_eps, rope_type=cfg.rope_type)
+        P.attn(L.pages, q, self.table, self.pos, 1, cfg.num_heads, cfg.attn_scale(), window=cfg.sliding_window, out=att, scratch=self.kv_scratch)
+
+    def paged_prompt(self, L: _Layer, qkv, q, att):
+        """The same for the rows of a portion of a prompt: ``prompt_count`` rows of every sequence from ``pos`` on."""
+        cfg, T = self.cfg, self.prefill_chunk
+        rows = dict(first=self.prompt_first, count=self.prompt_count)
+        P.append(L.pages, qkv, self.table, self.pos, T, self.cos_sin, cfg.num_heads, q_out=q, qw=L.qn, kw=L.kn, eps=cfg.rms_eps, rope_type=cfg.rope_type, **rows)
+        P.attn(L.pages, q, self.table, self.pos, T, cfg.num_heads, cfg.attn_scale(), window=cfg.sliding_window, out=att, scratch=self.kv_scratch, **rows)
+
     # ------------------------------------------------------------------ one decode step (captured)
     def _layer_step(self, L: _Layer, x_in, x_out):
         cfg = self.cfg
@@ -262,10 +323,13 @@ class InferenceEngine(TokenLoop):
         bf = self.dt == torch.bfloat16
         if self.fused:
             D.gemv_norm(L.wqkv, x_in, L.attn_norm, cfg.rms_eps, self.qkv, bf)
-            D.qk_rope_append(self.qkv, self.qk, L.qn, L.kn, self.cos_sin, self.pos, L.cK, L.cV, self.slot_pos, self.state,
-                             Hh, KV, hd, self.cap, PINNED_TOKENS, cfg.rms_eps, cfg.rope_type)
-            D.decode_attn(self.qk[:, :qd], L.cK, L.cV, self.slot_pos, self.state, self.att, self.att_scratch, self.splits,
-                          Hh, KV, hd, self.cap, cfg.sliding_window, cfg.attn_scale(), early=True)
+            if self.paged:
+                self.paged_step(L, self.qkv, self.qk[:, :qd], self.att)
+            else:
+                D.qk_rope_append(self.qkv, self.qk, L.qn, L.kn, self.cos_sin, self.pos, L.cK, L.cV, self.slot_pos, self.state,
+                                 Hh, KV, hd, self.cap, PINNED_TOKENS, cfg.rms_eps, cfg.rope_type)
+                D.decode_attn(self.qk[:, :qd], L.cK, L.cV, self.slot_pos, self.state, self.att, self.att_scratch, self.splits,
+                              Hh, KV, hd, self.cap, cfg.sliding_window, cfg.attn_scale(), early=True)
             D.gemv(L.wo, self.att, self.x_mid, addend=x_in)
             if cfg.use_moe:
                 D.route_norm(self.x_mid, L.ffn_norm, cfg.rms_eps, L.router, L.bias, cfg.moe_top_k, self.r_idx, self.r_w, bf)
@@ -279,10 +343,13 @@ class InferenceEngine(TokenLoop):
             return
         K.rmsnorm_fwd(x_in, L.attn_norm, self.xb, self.rr, cfg.rms_eps)
         D.gemv(L.wqkv, self.xb, self.qkv)
-        K.qk_norm_rope_fwd(self.qkv, self.qk, L.qn, L.kn, self.cos_sin, self.pos, Hh, KV, hd, cfg.rms_eps, cfg.rope_type)
-        D.kv_append(self.qk[:, qd:], self.qkv[:, qd + kvd:], L.cK, L.cV, self.slot_pos, self.state, self.cap, PINNED_TOKENS)
-        D.decode_attn(self.qk[:, :qd], L.cK, L.cV, self.slot_pos, self.state, self.att, self.att_scratch, self.splits,
-                      Hh, KV, hd, self.cap, cfg.sliding_window, cfg.attn_scale(), early=True)
+        if self.paged:
+            self.paged_step(L, self.qkv, self.qk[:, :qd], self.att)
+        else:
+            K.qk_norm_rope_fwd(self.qkv, self.qk, L.qn, L.kn, self.cos_sin, self.pos, Hh, KV, hd, cfg.rms_eps, cfg.rope_type)
+            D.kv_append(self.qk[:, qd:], self.qkv[:, qd + kvd:], L.cK, L.cV, self.slot_pos, self.state, self.cap, PINNED_TOKENS)
+            D.decode_attn(self.qk[:, :qd], L.cK, L.cV, self.slot_pos, self.state, self.att, self.att_scratch, self.splits,
+                          Hh, KV, hd, self.cap, cfg.sliding_window, cfg.attn_scale(), early=True)
         D.gemv(L.wo, self.att, self.x_mid, addend=x_in)
         K.rmsnorm_fwd(self.x_mid, L.ffn_norm, self.xb, self.rr, cfg.rms_eps)
         if cfg.use_moe:
@@ -297,6 +364,8 @@ class InferenceEngine(TokenLoop):
     def _forward_token(self):
         """Embedding of ``cur_tok`` through all layers to fp32 logits; advances the per-sequence state."""
         cfg = self.cfg
+        if not self._claimed:
+            self._claim(1)
         if self.mega is not None:
             try:
                 D.decode_mega(self.mega)
@@ -368,6 +437,8 @@ class InferenceEngine(TokenLoop):
         B, n = prompts.shape
         if B != self.B or n < 1:
             raise ValueError("prefill needs [%d, n >= 1] token ids, got %s" % (self.B, tuple(prompts.shape)))
+        if self.paged and n > self.cap:
+            raise ValueError("a prompt of %d tokens for an engine sized for %d" % (n, self.cap))
         prompts = prompts.to(self.dev, dtype=torch.int32)
         keep = min(n, self.hist_cap)                       # the penalty window looks at the most recent tokens only
         self.history[:, :keep].copy_(prompts[:, n - keep:])
@@ -375,7 +446,9 @@ class InferenceEngine(TokenLoop):
         # A prompt longer than the cache goes token by token: the ring keeps the first tokens and the most recent ones
         # (inference/kv_cache.h:11-106 in the reference), which the batched pass cannot express.
         head = min(n - 1, self.prefill_chunk) if (n - 1 >= 64 and n <= self.cap) else 0
-        if head > 0:
+        if self.paged:
+            head = self._prefill_paged(prompts)
+        elif head > 0:
             m = self._prefill_net()
             T = self.prefill_chunk
             ids = torch.zeros(B, T, dtype=torch.int32, device=self.dev)
@@ -390,3 +463,25 @@ class InferenceEngine(TokenLoop):
             self.cur_tok.copy_(prompts[:, j])
             self._forward_token()
         # logits of the last prompt token are in self.logits; cur_tok is set by the first sample call
+
+    def _prefill_paged(self, prompts) -> int:
+        """The batched pass over portions of ``prefill_chunk`` tokens, each attending to the pages of those before it; how many tokens went through it (fewer
+        than 64 that are left, and the last one, are the token step's)."""
+        B, n = prompts.shape
+        T, at = self.prefill_chunk, 0
+        self.state[:, :3] = 0
+        self.pos.zero_()
+        self._len = 0
+        while n - 1 - at >= 64:
+            m, c = self._prefill_net(), min(n - 1 - at, T)
+            ids = torch.zeros(B, T, dtype=torch.int32, device=self.dev)
+            ids[:, :c] = prompts[:, at:at + c]
+            m.ids.copy_(ids.view(-1))
+            self.prompt_count.fill_(c)
+            self._claim(c)
+            self._prompt_pass(m)
+            at += c
+            self.pos.fill_(at)
+        self.state[:, 0] = at
+        self.state[:, 1] = at
+        return at

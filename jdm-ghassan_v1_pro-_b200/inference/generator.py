@@ -92,6 +92,8 @@ class Generator:
             toks, reasons = self._run_host(sp, ids, max_new, stop_ids, stop_strings, on_text)
         if not host_only:
             torch.cuda.synchronize()
+        if getattr(eng, "paged", False):                      # keys that 8 bits could not hold, for one
+            eng.check()
         t2 = time.perf_counter()
         res = GenerationResult(tokens=toks, prompt_tokens=n, prefill_seconds=t1 - t0, decode_seconds=t2 - t1,
                                stopped=reasons)

@@ -75,11 +75,15 @@ def quant_name(m: LoadedModel) -> str:
     return "fp32"
 
 
-def build_engine(m: LoadedModel, batch: int = 1, max_len: int = 2048, fmt: str = "auto", prefill_chunk: int = 1024):
+def build_engine(m: LoadedModel, batch: int = 1, max_len: int = 2048, fmt: str = "auto", prefill_chunk: int = 1024,
+                 kv_cache: str = "16bit"):
     """Engine whose decode weights keep the file's storage format where the kernels read it directly; on a host without
     a CUDA device the fp32 CPU engine (`cpu_engine.CpuEngine`) over the expanded weights.  Layer-list models run on the
-    device only, in bfloat16 (``fmt`` "auto" / "bf16") or true fp32 ("f32")."""
+    device only, in bfloat16 (``fmt`` "auto" / "bf16") or true fp32 ("f32").  ``kv_cache`` "q8": keys and values in pages of 8 bits (decoders on the
+    device)."""
     import torch
+    if kv_cache != "16bit" and (isinstance(m.cfg, LayerListConfig) or not torch.cuda.is_available()):
+        raise ValueError("kv_cache %s is for decoder models on a CUDA device" % kv_cache)
     if isinstance(m.cfg, LayerListConfig):
         if not torch.cuda.is_available():
             raise RuntimeError("%s models run on a CUDA device only" % m.cfg.architecture)
@@ -97,4 +101,4 @@ def build_engine(m: LoadedModel, batch: int = 1, max_len: int = 2048, fmt: str =
         fmt = {"int8": "q8_64", "int4": "q4_0"}.get(quant_name(m), "f16")      # .gai block formats
     return InferenceEngine(m.cfg, m.named, fmt=fmt, batch=batch, max_len=min(max_len, max(64, m.cfg.max_seq_len)),
                            prefill_chunk=min(prefill_chunk, max_len), moe_bias=m.moe_bias or None, raw=raw,
-                           raw_types=m.tensor_types if raw is not None else None)
+                           raw_types=m.tensor_types if raw is not None else None, kv_cache=kv_cache)

@@ -274,7 +274,7 @@ class CudaModel:
             b = _LayerBuf()
             b.xb, b.rrms1 = CA.empty(N, d, **c16), CA.empty(N, **f32)
             b.qkv, b.qk = CA.empty(N, qd + 2 * kvd, **c16), CA.empty(N, qd + kvd, **c16)
-            b.att, b.lse = CA.empty(N, qd, **c16), CA.empty(N, H, **f32)
+            b.att, b.lse = (CA.empty if train else CA.zeros)(N, qd, **c16), CA.empty(N, H, **f32)
             b.x_mid = CA.empty(N, d, **f32)
             b.xb2, b.rrms2 = CA.empty(N, d, **c16), CA.empty(N, **f32)
             if cfg.use_moe:
@@ -396,10 +396,13 @@ class CudaModel:
             #                    query attends over the cache; everything else in this layer is the batched pass
             from ..ops import decode as D
             Lc = dec.layers[l]
-            D.qk_rope_append(b.qkv, b.qk, qw, kw, dec.cos_sin, dec.pos, Lc.cK, Lc.cV, dec.slot_pos, dec.state, H, KV, hd,
-                             dec.cap, dec.pinned, cfg.rms_eps, cfg.rope_type)
-            D.decode_attn(b.qk[:, :qd], Lc.cK, Lc.cV, dec.slot_pos, dec.state, b.att, dec.att_scratch, dec.splits, H, KV, hd,
-                          dec.cap, cfg.sliding_window, cfg.attn_scale(), early=True)
+            if dec.paged:
+                dec.paged_step(Lc, b.qkv, b.qk[:, :qd], b.att)
+            else:
+                D.qk_rope_append(b.qkv, b.qk, qw, kw, dec.cos_sin, dec.pos, Lc.cK, Lc.cV, dec.slot_pos, dec.state, H, KV, hd,
+                                 dec.cap, dec.pinned, cfg.rms_eps, cfg.rope_type)
+                D.decode_attn(b.qk[:, :qd], Lc.cK, Lc.cV, dec.slot_pos, dec.state, b.att, dec.att_scratch, dec.splits, H, KV, hd,
+                              dec.cap, cfg.sliding_window, cfg.attn_scale(), early=True)
         else:
             self._attention_forward(l, b, qw, kw)
         G.gemm(b.att, self.w16(p + "wo"), out=b.x_mid, addend=x_in, b_static=dec is not None)
@@ -415,8 +418,11 @@ class CudaModel:
     def _attention_forward(self, l: int, b: _LayerBuf, qw, kw):
         cfg = self.cfg
         qd, kvd, H, KV, hd = cfg.q_dim, cfg.kv_dim, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
-        K.qk_norm_rope_fwd(b.qkv, b.qk, qw, kw, self.cos_sin, self.pos, H, KV, hd, cfg.rms_eps, cfg.rope_type)
         sink = getattr(self, "kv_sink", None)
+        if sink is not None and sink.paged:      # rows past the prompt are not written: what is there is finite (zeros, or an earlier prompt's rows)
+            sink.paged_prompt(sink.layers[l], b.qkv, b.qk[:, :qd], b.att)
+            return
+        K.qk_norm_rope_fwd(b.qkv, b.qk, qw, kw, self.cos_sin, self.pos, H, KV, hd, cfg.rms_eps, cfg.rope_type)
         if sink is not None:   # prompt pass of the inference engine: keep this layer's keys (after RoPE) and values
             from ..ops import decode as D
             D.kv_rows(b.qk[:, qd:], b.qkv[:, qd + kvd:], sink.layers[l].cK, sink.layers[l].cV, sink.slot_pos, sink.prompt_len, self.T)
