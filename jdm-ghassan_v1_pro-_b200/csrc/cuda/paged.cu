@@ -1,7 +1,8 @@
 // Appending to and reading from the paged 8-bit cache (interface in gb_paged.h).
 //
 // A page of a head is one block's: it sees all numbers that share a scale, and nobody else writes to the page, so nothing here needs an atomic or a second pass over
-// memory.  The block also rotates the query heads of its key head, which reads every row of the input once and looks positions up where they are known.
+// memory.  A page's rows of a query head are another block's, so that all of a block's loads are on their way before it waits for any: with the query heads in the loop of
+// their key head's block, a page at a time, six prompts of 7.7 thousand tokens (32/8 heads of 128) took twice as long.
 #include <algorithm>
 
 #include "paged_util.cuh"
@@ -17,18 +18,19 @@ __device__ __forceinline__ float pg_scale(float amax) {
 // 1 / s of a power of two between 2^-120 and 2^122
 __device__ __forceinline__ float pg_inv(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-constexpr int PA_THREADS = 256;
+constexpr int PA_THREADS = 256, PA_FEW = 64;             // threads of a block; with few new tokens a sequence
 
-// Blocks: (sequence, page of its new tokens, key head).  HD / 16 lanes take a row: each the 8 pairs 8c ... 8c + 7 that a rotation turns, as two vectors of 8 numbers.
-template <typename T, int HD, int ROPE>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ qkv, long long ld, int H,
-                                                                  T* __restrict__ q_out, long long ld_q, const float* __restrict__ qw,
-                                                                  const float* __restrict__ kw, float eps, const float* __restrict__ cs, int positions) {
-  constexpr int LPR = HD / 16, RPP = PA_THREADS / LPR, PASSES = (PG + RPP - 1) / RPP, LDV = PG + 8;
+// Blocks: (page of the new tokens, key head or, from KV on, query head, sequence).  HD / 16 lanes take a row: each the 8 pairs 8c ... 8c + 7 that a rotation turns, as two
+// vectors of 8 numbers.  NT threads take ROWS rows, all of a page's or, with PA_FEW, at most PA_FEW * 16 / HD.
+template <typename T, int HD, int ROPE, int NT>
+__global__ void __launch_bounds__(NT) paged_append_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ qkv, long long ld, int H,
+                                                          T* __restrict__ q_out, long long ld_q, const float* __restrict__ qw,
+                                                          const float* __restrict__ kw, float eps, const float* __restrict__ cs, int positions) {
+  constexpr int LPR = HD / 16, RPP = NT / LPR, ROWS = NT == PA_FEW && RPP < PG ? RPP : PG, PASSES = (ROWS + RPP - 1) / RPP, LDV = PG + 8;
   __shared__ __align__(16) signed char sv[HD * LDV];
-  __shared__ float red[2][PA_THREADS / 32];
+  __shared__ float red[2][NT / 32];
   pdl_wait();
-  const int b = blockIdx.z, g = blockIdx.y, G = H / a.KV;
+  const int b = blockIdx.z, g = blockIdx.y;
   const PgSeq s = pg_seq(a, b);
   const int p = s.start / PG + (int)blockIdx.x;
   const int lo = max(s.start, p * PG), hi = min(s.start + s.n, (p + 1) * PG);      // positions of this block
@@ -37,7 +39,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     if (threadIdx.x == 0) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
     return;
   }
-  const int id = pg_page(a, b, p);
   const int n = hi - lo, off = lo - p * PG;
   const long long row0 = s.first + (lo - s.start);
   const int c = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
@@ -69,19 +70,45 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     }
   };
 
+  if (g >= a.KV) {                                       // a query head
+    const int h = g - a.KV;
+    float x[PASSES][16];
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const T* src = qkv + (row0 + min(ps * RPP + r0, n - 1)) * ld + (long long)h * HD;
+      pg_load8(src + o0, x[ps]);
+      pg_load8(src + o1, x[ps] + 8);
+    }
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const int r = ps * RPP + r0;
+      turn(x[ps], qw, lo + min(r, n - 1));
+      if (r >= n) continue;
+      T* dst = q_out + (row0 + r) * ld_q + (long long)h * HD;
+      pg_store8(dst + o0, x[ps]);
+      pg_store8(dst + o1, x[ps] + 8);
+    }
+    return;
+  }
+
+  const int id = pg_page(a, b, p);
   float ky[PASSES][16], vy[PASSES][16], km = 0.f, vm = 0.f;
   bool bad = false;
 #pragma unroll
   for (int ps = 0; ps < PASSES; ++ps) {
     const int r = ps * RPP + r0;
-    const bool on = r < n;
-    const T* src = qkv + (row0 + (on ? r : 0)) * ld;
+    const T* src = qkv + (row0 + min(r, n - 1)) * ld;
     const T *kp = src + (long long)(H + g) * HD, *vp = src + (long long)(H + a.KV + g) * HD;
     pg_load8(kp + o0, ky[ps]);
     pg_load8(kp + o1, ky[ps] + 8);
     pg_load8(vp + o0, vy[ps]);
     pg_load8(vp + o1, vy[ps] + 8);
-    turn(ky[ps], kw, lo + (on ? r : 0));
+  }
+#pragma unroll
+  for (int ps = 0; ps < PASSES; ++ps) {
+    const int r = ps * RPP + r0;
+    const bool on = r < n;
+    turn(ky[ps], kw, lo + min(r, n - 1));
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if (!(fabsf(ky[ps][i]) <= 3.402823466e38f)) { ky[ps][i] = 0.f; bad |= on; }
@@ -94,35 +121,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   vm = warp_max(vm);
   if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = km; red[1][threadIdx.x >> 5] = vm; }
 
-  // the query heads while the maxima meet
-  for (int i = r0; i < n * G; i += RPP) {
-    const int t = i / G, h = g * G + i - t * G;
-    float x[16];
-    const T* src = qkv + (row0 + t) * ld + (long long)h * HD;
-    pg_load8(src + o0, x);
-    pg_load8(src + o1, x + 8);
-    if (qw) {                                            // a row's lanes norm together: those past the end went home, so the mask is theirs
-      float ss = 0.f;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) ss += x[k] * x[k];
-      const unsigned mine = ((1u << LPR) - 1u) << ((threadIdx.x & 31) / LPR * LPR);
-#pragma unroll
-      for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(mine, ss, o);
-      float inv = rsqrtf(ss / (float)HD + eps);
-      if (!isfinite(inv)) inv = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) { x[k] *= inv * qw[o0 + k]; x[8 + k] *= inv * qw[o1 + k]; }
-    }
-    turn(x, nullptr, lo + t);
-    T* dst = q_out + (row0 + t) * ld_q + (long long)h * HD;
-    pg_store8(dst + o0, x);
-    pg_store8(dst + o1, x + 8);
-  }
   __syncthreads();
   if (id < 0) return;
   km = vm = 0.f;
 #pragma unroll
-  for (int w = 0; w < PA_THREADS / 32; ++w) { km = fmaxf(km, red[0][w]); vm = fmaxf(vm, red[1][w]); }
+  for (int w = 0; w < NT / 32; ++w) { km = fmaxf(km, red[0][w]); vm = fmaxf(vm, red[1][w]); }
   const long long at = (long long)id * a.KV + g;
   signed char *kc = a.k + at * PG * HD, *vc = a.v + at * PG * HD;
   float ks = pg_scale(km), vs = pg_scale(vm);
@@ -132,11 +135,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     vs = fmaxf(vs, vo);
     if (ks > ko) {
       const float r = ko * pg_inv(ks);
-      for (int i = threadIdx.x; i < off * HD; i += PA_THREADS) kc[i] = (signed char)__float2int_rn((float)kc[i] * r);
+      for (int i = threadIdx.x; i < off * HD; i += NT) kc[i] = (signed char)__float2int_rn((float)kc[i] * r);
     }
     if (vs > vo) {
       const float r = vo * pg_inv(vs);
-      for (int i = threadIdx.x; i < off * HD; i += PA_THREADS) {
+      for (int i = threadIdx.x; i < off * HD; i += NT) {
         signed char* q = vc + (i / off) * PG + i % off;
         *q = (signed char)__float2int_rn((float)*q * r);
       }
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   __syncthreads();
   // columns off ... off + n - 1 of every dimension: whole groups of 8 tokens at once, the edges one by one
   const int g0 = off / 8, ng = (off + n + 7) / 8 - g0;
-  for (int i = threadIdx.x; i < HD * ng; i += PA_THREADS) {
+  for (int i = threadIdx.x; i < HD * ng; i += NT) {
     const int d = i / ng, c0 = (g0 + i - d * ng) * 8;
     const signed char* src = sv + d * LDV + c0;
     signed char* dst = vc + d * PG + c0;
@@ -173,11 +176,20 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   }
 }
 
+// 4 codes as numbers: the byte, raised by 128, under the exponent of 2^23.  (Conversions of integers run at a quarter of this rate.)
+__device__ __forceinline__ void pg_numbers(uint32_t w, float scale, float* x) {
+  const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f) * scale;
+}
+
+// A block has a page of a head.  No shared memory: keys are rows already; of the values a thread takes 4 tokens of HD / 8 dimensions, a word each, and turns them byte by
+// byte, and neighbours fetch the rest of the sectors.
+constexpr int PR_THREADS = 128;
 template <typename T, int HD>
-__global__ void __launch_bounds__(PA_THREADS) paged_read_kernel(const __grid_constant__ gb_paged a, T* __restrict__ k_out, long long ld_k,
+__global__ void __launch_bounds__(PR_THREADS) paged_read_kernel(const __grid_constant__ gb_paged a, T* __restrict__ k_out, long long ld_k,
                                                                 T* __restrict__ v_out, long long ld_v) {
-  constexpr int CH = HD / 16, LDV = PG + 16;
-  __shared__ __align__(16) signed char sv[HD * LDV];
+  constexpr int CH = HD / 16, NK = PG * CH / PR_THREADS, UD = HD / 8;
   pdl_wait();
   const int b = blockIdx.z, g = blockIdx.y;
   const PgSeq s = pg_seq(a, b);
@@ -189,26 +201,67 @@ __global__ void __launch_bounds__(PA_THREADS) paged_read_kernel(const __grid_con
   const int n = hi - lo, off = lo - p * PG;
   const long long row0 = s.first + (lo - s.start), at = (long long)id * a.KV + g;
   const signed char *kc = a.k + at * PG * HD, *vc = a.v + at * PG * HD;
+  uint4 kw[NK];
+  uint32_t vw[UD];
+  const int d0 = (threadIdx.x & 7) * UD, t0 = (threadIdx.x >> 3) * 4;
+#pragma unroll
+  for (int j = 0; j < NK; ++j) kw[j] = reinterpret_cast<const uint4*>(kc)[j * PR_THREADS + threadIdx.x];
+#pragma unroll
+  for (int j = 0; j < UD; ++j) vw[j] = *reinterpret_cast<const uint32_t*>(vc + (d0 + j) * PG + t0);
   const float ks = a.ks[at], vs = a.vs[at];
-  constexpr float top = PgTop<T>::value;
-  for (int i = threadIdx.x; i < HD * 4; i += PA_THREADS)
-    *reinterpret_cast<uint4*>(sv + (i >> 2) * LDV + (i & 3) * 16) = *reinterpret_cast<const uint4*>(vc + i * 16);
-  __syncthreads();
-  for (int i = threadIdx.x; i < n * CH; i += PA_THREADS) {
-    const int t = i / CH, d0 = (i - t * CH) * 16;
-    const uint4 u = *reinterpret_cast<const uint4*>(kc + (off + t) * HD + d0);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float x[16];
+  const float top = PgTop<T>::value;
+  const bool clip = !(127.f * fmaxf(ks, vs) <= top);
+  auto put = [&](T* dst, float (&x)[8], int n8) {
+    if (clip) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = fminf(fmaxf((float)(signed char)(w[j >> 2] >> (8 * (j & 3))) * ks, -top), top);
-    T* dk = k_out + (row0 + t) * ld_k + (long long)g * HD + d0;
-    pg_store8(dk, x);
-    pg_store8(dk + 8, x + 8);
+      for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -top), top);
+    }
+    if (n8 == 8) pg_store8(dst, x);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(Cvt<T>::pack2(x[0], x[1]), Cvt<T>::pack2(x[2], x[3]));
+  };
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = fminf(fmaxf((float)sv[(d0 + j) * LDV + off + t] * vs, -top), top);
-    T* dv = v_out + (row0 + t) * ld_v + (long long)g * HD + d0;
-    pg_store8(dv, x);
-    pg_store8(dv + 8, x + 8);
+  for (int j = 0; j < NK; ++j) {
+    const int i = j * PR_THREADS + threadIdx.x, t = i / CH, r = t - off;
+    if (r < 0 || r >= n) continue;
+    T* dk = k_out + (row0 + r) * ld_k + (long long)g * HD + (i - t * CH) * 16;
+    float x[8], y[8];
+    pg_numbers(kw[j].x, ks, x);
+    pg_numbers(kw[j].y, ks, x + 4);
+    pg_numbers(kw[j].z, ks, y);
+    pg_numbers(kw[j].w, ks, y + 4);
+    put(dk, x, 8);
+    put(dk + 8, y, 8);
+  }
+  // word j: dimension d0 + j of tokens t0 ... t0 + 3; turned: word q of a token: its dimensions d0 + 4q ... d0 + 4q + 3
+  uint32_t tw[4][UD / 4];
+#pragma unroll
+  for (int q = 0; q < UD / 4; ++q) {
+    const uint32_t a0 = __byte_perm(vw[4 * q], vw[4 * q + 1], 0x5140), a1 = __byte_perm(vw[4 * q], vw[4 * q + 1], 0x7362);
+    const uint32_t b0 = __byte_perm(vw[4 * q + 2], vw[4 * q + 3], 0x5140), b1 = __byte_perm(vw[4 * q + 2], vw[4 * q + 3], 0x7362);
+    tw[0][q] = __byte_perm(a0, b0, 0x5410);
+    tw[1][q] = __byte_perm(a0, b0, 0x7632);
+    tw[2][q] = __byte_perm(a1, b1, 0x5410);
+    tw[3][q] = __byte_perm(a1, b1, 0x7632);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = t0 + k - off;
+    if (r < 0 || r >= n) continue;
+    T* dv = v_out + (row0 + r) * ld_v + (long long)g * HD + d0;
+    float x[8];
+    if constexpr (UD == 4) {
+      pg_numbers(tw[k][0], vs, x);
+#pragma unroll
+      for (int i = 4; i < 8; ++i) x[i] = 0.f;
+      put(dv, x, 4);
+    } else {
+#pragma unroll
+      for (int q = 0; q < UD / 8; ++q) {
+        pg_numbers(tw[k][2 * q], vs, x);
+        pg_numbers(tw[k][2 * q + 1], vs, x + 4);
+        put(dv + 8 * q, x, 8);
+      }
+    }
   }
 }
 
@@ -242,8 +295,14 @@ extern "C" int gb_paged_append(const gb_paged* a, const void* qkv, long long ld_
   if (!gb_paged_rows_ok(qkv, ld_qkv, (long long)(H + 2 * a->KV) * a->hd) || !gb_paged_rows_ok(q_out, ld_q, (long long)H * a->hd)) return -4;
   dim3 grid;
   if (const int rc = gb_paged_grid(a, &grid)) return rc;
-#define CALL(T, HD) \
-  GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE>), grid, dim3(PA_THREADS), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions)
+  grid.y += H;
+  if (grid.y > 65535) return -3;
+  const bool few = a->max_new <= PA_FEW * 16 / a->hd;
+#define CALL(T, HD)                                                                                                                                                 \
+  do {                                                                                                                                                              \
+    if (few) GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, PA_FEW>), grid, dim3(PA_FEW), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
+    else GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, PA_THREADS>), grid, dim3(PA_THREADS), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
+  } while (0)
   if (rope_type == 0) {
     constexpr int ROPE = 0;
     GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
@@ -262,7 +321,7 @@ extern "C" int gb_paged_read(const gb_paged* a, void* k_out, long long ld_k, voi
   if (!gb_paged_rows_ok(k_out, ld_k, width) || !gb_paged_rows_ok(v_out, ld_v, width)) return -4;
   dim3 grid;
   if (const int rc = gb_paged_grid(a, &grid)) return rc;
-#define CALL(T, HD) GB_PDL_LAUNCH((paged_read_kernel<T, HD>), grid, dim3(PA_THREADS), st, *a, (T*)k_out, ld_k, (T*)v_out, ld_v)
+#define CALL(T, HD) GB_PDL_LAUNCH((paged_read_kernel<T, HD>), grid, dim3(PR_THREADS), st, *a, (T*)k_out, ld_k, (T*)v_out, ld_v)
   GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
 #undef CALL
   return gb_launch_rc();
