@@ -18,34 +18,62 @@ __device__ __forceinline__ float pg_scale(float amax) {
 // 1 / s of a power of two between 2^-120 and 2^122
 __device__ __forceinline__ float pg_inv(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-constexpr int PA_THREADS = 256, PA_FEW = 64;             // threads of a block; with few new tokens a sequence
+// 4 codes as numbers: the byte, raised by 128, under the exponent of 2^23.  (Conversions of integers run at a quarter of this rate.)
+__device__ __forceinline__ void pg_numbers(uint32_t w, float scale, float* x) {
+  const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f) * scale;
+}
 
-// Blocks: (page of the new tokens, key head or, from KV on, query head, sequence).  HD / 16 lanes take a row: each the 8 pairs 8c ... 8c + 7 that a rotation turns, as two
-// vectors of 8 numbers.  NT threads take ROWS rows, all of a page's or, with PA_FEW, at most PA_FEW * 16 / HD.
+// 4 numbers of at most 127 as codes, rounded to the nearest (even) integer: that is what is left in the low byte of x + 1.5 * 2^23.
+__device__ __forceinline__ uint32_t pg_codes(const float* x, float inv) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(x[i], inv, 12582912.f));
+  return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+}
+
+constexpr int PA_FEW = 64;                               // threads of a block with few new tokens a sequence: PA_FEW * 16 / HD at most
+
+// Blocks: (key head, behind them two query heads each; page of the new tokens; sequence): neighbours read neighbouring parts of the same rows.  HD / 16 lanes take a row:
+// each the 8 pairs 8c ... 8c + 7 that a rotation turns, as two vectors of 8 numbers.  4 HD threads have a page's 64 tokens at once, which 64 registers
+// allow; half the threads with two rows each took 114, two blocks an SM.  Bound by instructions issued as much as by memory: codes are rounded by an addition
+// and not by conversions, a page's values are turned in registers, four tokens to a word, not stored byte by byte.
 template <typename T, int HD, int ROPE, int NT>
-__global__ void __launch_bounds__(NT) paged_append_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ qkv, long long ld, int H,
+__global__ void __launch_bounds__(NT, NT == PA_FEW ? 8 : 1024 / NT) paged_append_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ qkv, long long ld, int H,
                                                           T* __restrict__ q_out, long long ld_q, const float* __restrict__ qw,
                                                           const float* __restrict__ kw, float eps, const float* __restrict__ cs, int positions) {
-  constexpr int LPR = HD / 16, RPP = NT / LPR, ROWS = NT == PA_FEW && RPP < PG ? RPP : PG, PASSES = (ROWS + RPP - 1) / RPP, LDV = PG + 8;
-  __shared__ __align__(16) signed char sv[HD * LDV];
-  __shared__ float red[2][NT / 32];
+  constexpr bool FEW = NT != 4 * HD;
+  constexpr int LPR = HD / 16, LDV = PG + 4;
+  __shared__ __align__(16) uint32_t sv[FEW ? 1 : HD * LDV / 4];
+  __shared__ uint32_t red[2][NT / 32];
   pdl_wait();
-  const int b = blockIdx.z, g = blockIdx.y;
+  const int b = blockIdx.z, g = blockIdx.x;
   const PgSeq s = pg_seq(a, b);
-  const int p = s.start / PG + (int)blockIdx.x;
+  const int p = s.start / PG + (int)blockIdx.y;
   const int lo = max(s.start, p * PG), hi = min(s.start + s.n, (p + 1) * PG);      // positions of this block
   if (lo >= hi) return;
   if (hi > positions) {
     if (threadIdx.x == 0) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
     return;
   }
-  const int n = hi - lo, off = lo - p * PG;
-  const long long row0 = s.first + (lo - s.start);
-  const int c = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
+  const int n = hi - lo, off = lo - p * PG, c = threadIdx.x % LPR;
+  const int r = (int)threadIdx.x / LPR - (FEW ? 0 : off), slot = off + r;            // this thread's row of the block's n (if it is one), and its place in the page
+  const bool on = r >= 0 && r < n;
+  const int rr = min(max(r, 0), n - 1);
+  const long long row = s.first + (lo - s.start) + rr;
   const int o0 = ROPE == 0 ? 16 * c : 8 * c, o1 = ROPE == 0 ? 16 * c + 8 : HD / 2 + 8 * c;
+  const T* src = qkv + row * ld;
 
+  float co[8], si[8];
+  auto angles = [&]() {                                    // asked for with the row
+    const float4* cp = reinterpret_cast<const float4*>(cs + (long long)(lo + rr) * HD + 8 * c);
+    const float4 ca = cp[0], cb = cp[1], sa = cp[HD / 8], sb = cp[HD / 8 + 1];
+    co[0] = ca.x; co[1] = ca.y; co[2] = ca.z; co[3] = ca.w; co[4] = cb.x; co[5] = cb.y; co[6] = cb.z; co[7] = cb.w;
+    si[0] = sa.x; si[1] = sa.y; si[2] = sa.z; si[3] = sa.w; si[4] = sb.x; si[5] = sb.y; si[6] = sb.z; si[7] = sb.w;
+  };
   // x: the two vectors of a row; normed and turned
-  auto turn = [&](float* x, const float* w, int pos) {
+  auto turn = [&](float* x, const float* w) {
     if (w) {
       float ss = 0.f;
 #pragma unroll
@@ -57,10 +85,6 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 8; ++i) { x[i] *= inv * w[o0 + i]; x[8 + i] *= inv * w[o1 + i]; }
     }
-    const float4* cp = reinterpret_cast<const float4*>(cs + (long long)pos * HD + 8 * c);
-    const float4* sp = reinterpret_cast<const float4*>(cs + (long long)pos * HD + HD / 2 + 8 * c);
-    const float4 ca = cp[0], cb = cp[1], sa = sp[0], sb = sp[1];
-    const float co[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w}, si[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {                         // products and differences rounded one by one, as the definition has them
       const int i0 = ROPE == 0 ? 2 * i : i, i1 = ROPE == 0 ? 2 * i + 1 : 8 + i;
@@ -70,117 +94,128 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(const __grid_constant_
     }
   };
 
-  if (g >= a.KV) {                                       // a query head
-    const int h = g - a.KV;
-    float x[PASSES][16];
-#pragma unroll
-    for (int ps = 0; ps < PASSES; ++ps) {
-      const T* src = qkv + (row0 + min(ps * RPP + r0, n - 1)) * ld + (long long)h * HD;
-      pg_load8(src + o0, x[ps]);
-      pg_load8(src + o1, x[ps] + 8);
-    }
-#pragma unroll
-    for (int ps = 0; ps < PASSES; ++ps) {
-      const int r = ps * RPP + r0;
-      turn(x[ps], qw, lo + min(r, n - 1));
-      if (r >= n) continue;
-      T* dst = q_out + (row0 + r) * ld_q + (long long)h * HD;
-      pg_store8(dst + o0, x[ps]);
-      pg_store8(dst + o1, x[ps] + 8);
+  if (g >= a.KV) {                                       // query heads h, h + 1
+    const int h = 2 * (g - a.KV);
+    const bool two = h + 1 < H;
+    float x[16], y[16];
+    pg_load8(src + (long long)h * HD + o0, x);
+    pg_load8(src + (long long)h * HD + o1, x + 8);
+    pg_load8(src + (long long)(h + two) * HD + o0, y);
+    pg_load8(src + (long long)(h + two) * HD + o1, y + 8);
+    angles();
+    turn(x, qw);
+    turn(y, qw);
+    if (!on) return;
+    T* dst = q_out + row * ld_q + (long long)h * HD;
+    pg_store8(dst + o0, x);
+    pg_store8(dst + o1, x + 8);
+    if (two) {
+      pg_store8(dst + HD + o0, y);
+      pg_store8(dst + HD + o1, y + 8);
     }
     return;
   }
 
   const int id = pg_page(a, b, p);
-  float ky[PASSES][16], vy[PASSES][16], km = 0.f, vm = 0.f;
-  bool bad = false;
+  float ky[16], vy[16];
+  const T *kp = src + (long long)(H + g) * HD, *vp = src + (long long)(H + a.KV + g) * HD;
+  pg_load8(kp + o0, ky);
+  pg_load8(kp + o1, ky + 8);
+  pg_load8(vp + o0, vy);
+  pg_load8(vp + o1, vy + 8);
+  angles();
+  turn(ky, kw);
+  uint32_t km = 0, vm = 0;                               // largest sizes, as bits: what is not finite is larger than all that is
 #pragma unroll
-  for (int ps = 0; ps < PASSES; ++ps) {
-    const int r = ps * RPP + r0;
-    const T* src = qkv + (row0 + min(r, n - 1)) * ld;
-    const T *kp = src + (long long)(H + g) * HD, *vp = src + (long long)(H + a.KV + g) * HD;
-    pg_load8(kp + o0, ky[ps]);
-    pg_load8(kp + o1, ky[ps] + 8);
-    pg_load8(vp + o0, vy[ps]);
-    pg_load8(vp + o1, vy[ps] + 8);
+  for (int i = 0; i < 16; ++i) {
+    km = max(km, __float_as_uint(ky[i]) & 0x7fffffffu);
+    vm = max(vm, __float_as_uint(vy[i]) & 0x7fffffffu);
   }
-#pragma unroll
-  for (int ps = 0; ps < PASSES; ++ps) {
-    const int r = ps * RPP + r0;
-    const bool on = r < n;
-    turn(ky[ps], kw, lo + min(r, n - 1));
+  if (max(km, vm) >= 0x7f800000u) {
+    if (on) atomicCAS(a.status, 0, ST_NOT_FINITE);
+    km = vm = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      if (!(fabsf(ky[ps][i]) <= 3.402823466e38f)) { ky[ps][i] = 0.f; bad |= on; }
-      if (!(fabsf(vy[ps][i]) <= 3.402823466e38f)) { vy[ps][i] = 0.f; bad |= on; }
-      if (on) { km = fmaxf(km, fabsf(ky[ps][i])); vm = fmaxf(vm, fabsf(vy[ps][i])); }
+      const uint32_t ku = __float_as_uint(ky[i]) & 0x7fffffffu, vu = __float_as_uint(vy[i]) & 0x7fffffffu;
+      if (ku >= 0x7f800000u) ky[i] = 0.f; else km = max(km, ku);
+      if (vu >= 0x7f800000u) vy[i] = 0.f; else vm = max(vm, vu);
     }
   }
-  if (bad) atomicCAS(a.status, 0, ST_NOT_FINITE);
-  km = warp_max(km);
-  vm = warp_max(vm);
+  km = __reduce_max_sync(0xffffffffu, on ? km : 0u);
+  vm = __reduce_max_sync(0xffffffffu, on ? vm : 0u);
   if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = km; red[1][threadIdx.x >> 5] = vm; }
-
   __syncthreads();
   if (id < 0) return;
-  km = vm = 0.f;
+  km = vm = 0;
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) { km = fmaxf(km, red[0][w]); vm = fmaxf(vm, red[1][w]); }
+  for (int w = 0; w < NT / 32; ++w) { km = max(km, red[0][w]); vm = max(vm, red[1][w]); }
   const long long at = (long long)id * a.KV + g;
   signed char *kc = a.k + at * PG * HD, *vc = a.v + at * PG * HD;
-  float ks = pg_scale(km), vs = pg_scale(vm);
+  float ks = pg_scale(__uint_as_float(km)), vs = pg_scale(__uint_as_float(vm));
   if (off > 0) {                                         // tokens of earlier calls share the page
     const float ko = a.ks[at], vo = a.vs[at];
     ks = fmaxf(ks, ko);
     vs = fmaxf(vs, vo);
     if (ks > ko) {
-      const float r = ko * pg_inv(ks);
-      for (int i = threadIdx.x; i < off * HD; i += NT) kc[i] = (signed char)__float2int_rn((float)kc[i] * r);
-    }
-    if (vs > vo) {
-      const float r = vo * pg_inv(vs);
-      for (int i = threadIdx.x; i < off * HD; i += NT) {
-        signed char* q = vc + (i / off) * PG + i % off;
-        *q = (signed char)__float2int_rn((float)*q * r);
+      const float f = ko * pg_inv(ks);
+      uint32_t* w = reinterpret_cast<uint32_t*>(kc);
+      for (int i = threadIdx.x; i < off * (HD / 4); i += NT) {
+        float x[4];
+        pg_numbers(w[i], f, x);
+        w[i] = pg_codes(x, 1.f);
       }
     }
-    __syncthreads();                                     // the old scales are read
+    if (vs > vo) {
+      const float f = vo * pg_inv(vs);
+      uint32_t* w = reinterpret_cast<uint32_t*>(vc);
+      for (int i = threadIdx.x; i < HD * (PG / 4); i += NT) {
+        const int t = (i & 15) * 4;                      // this word's tokens: those from `off` on are the next call's, or nobody's
+        if (t >= off) continue;
+        float x[4];
+        pg_numbers(w[i], f, x);
+        const uint32_t mine = off - t >= 4 ? 0xffffffffu : (1u << (8 * (off - t))) - 1u;
+        w[i] = (pg_codes(x, 1.f) & mine) | (w[i] & ~mine);
+      }
+    }
+    __syncthreads();                                     // the old scales are read, the old codes written
   }
   if (threadIdx.x == 0) { a.ks[at] = ks; a.vs[at] = vs; }
   const float ki = pg_inv(ks), vi = pg_inv(vs);
-#pragma unroll
-  for (int ps = 0; ps < PASSES; ++ps) {
-    const int r = ps * RPP + r0;
-    if (r >= n) continue;
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i >> 2] |= (uint32_t)(__float2int_rn(ky[ps][i] * ki) & 255) << (8 * (i & 3));
-    signed char* kr = kc + (off + r) * HD;
-    *reinterpret_cast<uint2*>(kr + o0) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(kr + o1) = make_uint2(w[2], w[3]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sv[((i < 8 ? o0 : o1 - 8) + i) * LDV + off + r] = (signed char)__float2int_rn(vy[ps][i] * vi);
+  if (on) {
+    signed char* kr = kc + slot * HD;
+    *reinterpret_cast<uint2*>(kr + o0) = make_uint2(pg_codes(ky, ki), pg_codes(ky + 4, ki));
+    *reinterpret_cast<uint2*>(kr + o1) = make_uint2(pg_codes(ky + 8, ki), pg_codes(ky + 12, ki));
   }
-  __syncthreads();
-  // columns off ... off + n - 1 of every dimension: whole groups of 8 tokens at once, the edges one by one
-  const int g0 = off / 8, ng = (off + n + 7) / 8 - g0;
-  for (int i = threadIdx.x; i < HD * ng; i += NT) {
-    const int d = i / ng, c0 = (g0 + i - d * ng) * 8;
-    const signed char* src = sv + d * LDV + c0;
-    signed char* dst = vc + d * PG + c0;
-    if (c0 >= off && c0 + 8 <= off + n) {
-      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  if constexpr (FEW) {
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) vc[((i < 8 ? o0 : o1 - 8) + i) * PG + slot] = (signed char)__float_as_uint(fmaf(vy[i], vi, 12582912.f));
+    }
+  } else {
+    // word j of a lane: 4 dimensions of its token; the lanes of 4 tokens turn them, so that lane k has dimension k of the four and all tokens
+    const int k = (threadIdx.x / LPR) & 3, t4 = (int)threadIdx.x / LPR / 4;
+    const uint32_t one = k & 1 ? 0x3715u : 0x6240u, other = k & 2 ? 0x3276u : 0x5410u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w = pg_codes(vy + 4 * j, vi);
+      w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, LPR), one);
+      w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 2 * LPR), other);
+      sv[((j < 2 ? o0 + 4 * j : o1 + 4 * j - 8) + k) * (LDV / 4) + t4] = w;
+    }
+    __syncthreads();
+    // 16 tokens of a dimension a thread
+    const int d = threadIdx.x >> 2, t = (threadIdx.x & 3) * 16;
+    const uint32_t* from = sv + d * (LDV / 4) + t / 4;
+    const uint32_t w[4] = {from[0], from[1], from[2], from[3]};
+    signed char* dst = vc + d * PG + t;
+    if (t >= off && t + 16 <= off + n) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-      for (int j = max(c0, off) - c0; j < min(c0 + 8, off + n) - c0; ++j) dst[j] = src[j];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (t + j >= off && t + j < off + n) dst[j] = (signed char)(w[j >> 2] >> (8 * (j & 3)));
     }
   }
-}
-
-// 4 codes as numbers: the byte, raised by 128, under the exponent of 2^23.  (Conversions of integers run at a quarter of this rate.)
-__device__ __forceinline__ void pg_numbers(uint32_t w, float scale, float* x) {
-  const uint32_t u = w ^ 0x80808080u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f) * scale;
 }
 
 // A block has a page of a head.  No shared memory: keys are rows already; of the values a thread takes 4 tokens of HD / 8 dimensions, a word each, and turns them byte by
@@ -191,9 +226,9 @@ __global__ void __launch_bounds__(PR_THREADS) paged_read_kernel(const __grid_con
                                                                 T* __restrict__ v_out, long long ld_v) {
   constexpr int CH = HD / 16, NK = PG * CH / PR_THREADS, UD = HD / 8;
   pdl_wait();
-  const int b = blockIdx.z, g = blockIdx.y;
+  const int b = blockIdx.z, g = blockIdx.x;
   const PgSeq s = pg_seq(a, b);
-  const int p = s.start / PG + (int)blockIdx.x;
+  const int p = s.start / PG + (int)blockIdx.y;
   const int lo = max(s.start, p * PG), hi = min(s.start + s.n, (p + 1) * PG);
   if (lo >= hi) return;
   const int id = pg_page(a, b, p);
@@ -279,11 +314,11 @@ static bool gb_paged_rows_ok(const void* p, long long ld, long long width) {
     else { if (hd == 32) { CALL(__half, 32); } else if (hd == 64) { CALL(__half, 64); } else { CALL(__half, 128); } }     \
   } while (0)
 
-// Blocks along x: pages that max_new tokens can touch, wherever in a page they begin.
+// Blocks along y: pages that max_new tokens can touch, wherever in a page they begin.
 static int gb_paged_grid(const gb_paged* a, dim3* grid) {
   const int px = (int)std::min<long long>(((long long)a->max_new + 2 * GB_PAGE - 2) / GB_PAGE, a->W);
-  if (a->KV > 65535 || a->B > 65535) return -3;
-  *grid = dim3(px, a->KV, a->B);
+  if (px > 65535 || a->B > 65535) return -3;
+  *grid = dim3(a->KV, px, a->B);
   return 0;
 }
 
@@ -295,13 +330,12 @@ extern "C" int gb_paged_append(const gb_paged* a, const void* qkv, long long ld_
   if (!gb_paged_rows_ok(qkv, ld_qkv, (long long)(H + 2 * a->KV) * a->hd) || !gb_paged_rows_ok(q_out, ld_q, (long long)H * a->hd)) return -4;
   dim3 grid;
   if (const int rc = gb_paged_grid(a, &grid)) return rc;
-  grid.y += H;
-  if (grid.y > 65535) return -3;
+  grid.x += (H + 1) / 2;
   const bool few = a->max_new <= PA_FEW * 16 / a->hd;
 #define CALL(T, HD)                                                                                                                                                 \
   do {                                                                                                                                                              \
     if (few) GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, PA_FEW>), grid, dim3(PA_FEW), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
-    else GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, PA_THREADS>), grid, dim3(PA_THREADS), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
+    else GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, 4 * HD>), grid, dim3(4 * HD), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
   } while (0)
   if (rope_type == 0) {
     constexpr int ROPE = 0;
