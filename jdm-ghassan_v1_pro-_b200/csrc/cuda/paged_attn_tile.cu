@@ -5,7 +5,8 @@
 //
 // One block an SM: two warpgroups of soft-max threads, a row each, take turns with the tensor cores (while one finds its weights, the products of the other run); four warps expand the
 // pages, a tile of 128 keys at a time, from codes in global memory to float16 integers in the swizzled layout of the MMAs (integers up to 127 are exact, the scales go into the
-// soft-max: a key scale into the score's factor, a value scale into the weight's exponent, as in paged_attn_token.cu); one warp issues.  Scores and weights share tensor memory:
+// soft-max: a key scale into the score's factor, a value scale into the weight's exponent, as in paged_attn_token.cu); a warp for each warpgroup issues (one for both was busy
+// issuing and asking barriers all the time).  Scores and weights share tensor memory:
 // weights of a chunk of 32 columns go where scores that have been read were, and are the A operand of the second product from there.
 //
 // The work is dealt in key tiles: all (sequence, key head, item, key tile) in a row are cut into equal runs, one a block.  Items that a cut goes through leave records
@@ -17,20 +18,22 @@
 
 namespace gb {
 
-constexpr int TL_ROWS = 256, TL_KEYS = 128, TL_THREADS = 512;
+constexpr int TL_ROWS = 256, TL_THREADS = 512;
 constexpr float TL_OFF = 7.f, TL_LAZY = 8.f;   // weights are held as 2^7 of themselves and may grow 2^8 before the sums are rescaled
 
 template <int HD>
 struct Tl {
-  static constexpr int PANELS = HD <= 64 ? 1 : 2;             // 64 dimensions each
-  static constexpr int Q = 128 * 128 * PANELS, K = 128 * 128 * PANELS, V = 2 * HD * 128, STAGE = K + V;
-  static constexpr int STAGES = HD == 128 ? 2 : 3;
-  // columns of tensor memory: scores 0 and 128; at hd 128 the results take the other 256 and weights go over the scores, which then wait for the second product; else
-  // weights have places of their own and the next scores are found while the soft-max is still at work on these
+  // Tensor memory has 512 columns.  At hd 128 the results take 256: scores come in tiles of 64 keys, two buffers a warpgroup, and weights go over the scores; the products of a
+  // tile run while the soft-max is at work on the next (2048 tokens behind 14000, 32/8 heads, 558 us; tiles of 128 keys with one buffer, whose products a
+  // warpgroup waits for, 571).  Else tiles have 128 keys and one buffer, which is free once the scores are in registers, and weights have places of their own.
   static constexpr bool OVER = HD == 128;
-  static constexpr int P0 = OVER ? 0 : 256, P_STEP = OVER ? 128 : 64, O0 = OVER ? 256 : 384;
+  static constexpr int KEYS = OVER ? 64 : 128, PP = KEYS / PG, BUFS = OVER && KEYS == 64 ? 2 : 1;
+  static constexpr int P0 = OVER ? 0 : 256, O0 = OVER ? 256 : 384;
+  static constexpr int PANELS = HD <= 64 ? 1 : 2;             // 64 dimensions each
+  static constexpr int Q = 128 * 128 * PANELS, K = KEYS * 128 * PANELS, V = PP * HD * 128, STAGE = K + V;
+  static constexpr int STAGES = OVER ? 256 / KEYS : 3, AHEAD = 128 / KEYS;
   // registers a thread: soft-max, expanding, issuing; launched with 128, so 2 x 128 x S + 128 x (E + I) is at most 65536
-  static constexpr int REGS_S = 184, REGS_E = HD == 128 ? 104 : 88, REGS_I = HD == 128 ? 40 : 56;
+  static constexpr int REGS_S = OVER && KEYS == 128 ? 176 : 184, REGS_E = OVER && KEYS == 128 ? 104 : 88, REGS_I = 56;
   static constexpr int REC = TL_ROWS * (HD + 2);              // floats of a record: [HD / 4][256] four results, then [256] pairs (maximum, sum)
 };
 
@@ -58,20 +61,18 @@ __device__ __forceinline__ float2 tl_add2(float2 a, float2 b) {
   return d;
 }
 
-constexpr int TL_AHEAD = 1;
-struct TlItem {
-  int lo, n;                                                  // first key tile, number of them
-  // an item has n + TL_AHEAD places; those of a run that are its places k0 ... k1 - 1 are these key tiles
-  __device__ __forceinline__ int tile(int k) const { return max(0, k - TL_AHEAD); }
-};
+struct TlItem { int lo, n; };                                 // first key tile, number of them
+template <int KEYS>
 __device__ __forceinline__ TlItem tl_item(const PgAttn& p, const PgSeq& s, int G, int qt) {
   const int r1 = min(s.n * G, (qt + 1) * TL_ROWS) - 1;
   const int p0 = s.start + qt * TL_ROWS / G, p1 = s.start + r1 / G;
-  const int lo = p.window > 0 ? max(0, p0 - p.window + 1) / TL_KEYS : 0;
-  return {lo, p1 / TL_KEYS - lo + 1};
+  const int lo = p.window > 0 ? max(0, p0 - p.window + 1) / KEYS : 0;
+  return {lo, p1 / KEYS - lo + 1};
 }
 
-// A block's walk over its run: places f ... end, one piece of an item after the other.
+// A block's walk over its run: places f ... end, one piece of an item after the other.  An item has a place for each key tile and, ahead of them, AHEAD for its start and end: loading queries,
+// filling and emptying the pipelines take as long as a tile of 128 keys.
+template <int AHEAD>
 struct TlWalk {
   int f, end, b, g, qt, k;                                    // k: places of the item that come before place f
   PgSeq s;
@@ -82,14 +83,14 @@ struct TlWalk {
   }
   // the run's part of this item: key tiles k0 ... k1 - 1
   __device__ __forceinline__ void part(const TlItem& item, int& k0, int& k1) const {
-    k0 = item.tile(k);
-    k1 = item.tile(min(item.n + TL_AHEAD, k + end - f));
+    k0 = max(0, k - AHEAD);
+    k1 = max(0, min(item.n + AHEAD, k + end - f) - AHEAD);
   }
   __device__ __forceinline__ void next(const PgAttn& p, int G, const int* cum, const TlItem& item) {
-    const int taken = min(item.n + TL_AHEAD - k, end - f);
+    const int taken = min(item.n + AHEAD - k, end - f);
     f += taken;
     k += taken;
-    if (k < item.n + TL_AHEAD || f >= end) return;
+    if (k < item.n + AHEAD || f >= end) return;
     k = 0;
     if (++qt < tiles) return;
     qt = 0;
@@ -108,18 +109,19 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
   uint8_t *sQ = smem, *sKV = smem + 2 * L::Q;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + L::STAGES * L::STAGE);
   uint64_t *k_full = bars, *k_empty = k_full + L::STAGES, *v_full = k_empty + L::STAGES, *v_empty = v_full + L::STAGES;
-  uint64_t *s_full = v_empty + L::STAGES, *p_ready = s_full + 2, *o_full = s_full + 4, *q_full = s_full + 6, *s_free = s_full + 8, *turn = s_full + 10;
-  float4* scales = reinterpret_cast<float4*>(turn + 2);                       // of four key tiles (they outlive a stage): key scales of the two pages, value scales; a negative
+  uint64_t *s_full = v_empty + L::STAGES, *p_ready = s_full + 4, *o_full = s_full + 8, *q_full = s_full + 10, *s_free = s_full + 12, *turn = s_full + 14;   // s_full, p_ready: [2 wg + buffer]
+  float4* scales = reinterpret_cast<float4*>(turn + 2);                       // of eight key tiles (they outlive a stage): key scales of the two pages, value scales; a negative
                                                                               // key scale: no page
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scales + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scales + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* cum = reinterpret_cast<int*>(tmem_slot + 2);                           // key tiles (of one head) of the sequences before
   const gb_paged& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.H / a.KV;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L::STAGES; ++s) { mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 1); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 1); }
-    for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 2); mbar_init(&p_ready[w], 4); mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); mbar_init(&turn[w], 4); }
+    for (int s = 0; s < L::STAGES; ++s) { mbar_init(&k_full[s], 4); mbar_init(&k_empty[s], 2); mbar_init(&v_full[s], 4); mbar_init(&v_empty[s], 2); }
+    for (int w = 0; w < 4; ++w) { mbar_init(&s_full[w], 2); mbar_init(&p_ready[w], 4); }
+    for (int w = 0; w < 2; ++w) { mbar_init(&o_full[w], 1); mbar_init(&q_full[w], 4); mbar_init(&s_free[w], 4); mbar_init(&turn[w], 4); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
     const PgSeq s = pg_seq(a, b);
     const int tiles = (s.n * G + TL_ROWS - 1) / TL_ROWS;
     int n = 0;
-    for (int qt = lane; qt < tiles; qt += 32) n += tl_item(p, s, G, qt).n + TL_AHEAD;
+    for (int qt = lane; qt < tiles; qt += 32) n += tl_item<L::KEYS>(p, s, G, qt).n + L::AHEAD;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     if (lane == 0) cum[b + 1] = n;
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
   }
   __syncthreads();
   const int total = a.KV * cum[a.B], quota = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-  TlWalk start;
+  TlWalk<L::AHEAD> start;
   start.f = min(total, (int)blockIdx.x * quota);
   start.end = min(total, start.f + quota);
   TlDesc* desc = reinterpret_cast<TlDesc*>(p.part);
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
     start.qt = 0;
     start.k = 0;
     for (int q0 = 0; q0 < start.tiles; q0 += 32) {            // the item that holds place f: a warp looks through 32 at a time
-      const int n = q0 + lane < start.tiles ? tl_item(p, start.s, G, q0 + lane).n + TL_AHEAD : 0;
+      const int n = q0 + lane < start.tiles ? tl_item<L::KEYS>(p, start.s, G, q0 + lane).n + L::AHEAD : 0;
       int v = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -196,13 +198,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       // ------------------------------------------------------------------------------------------ soft-max: a thread a row
       const int wg = warp >> 2, r = threadIdx.x & 127;
       const uint32_t row = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t tS = tmem + wg * 128 + row, tP = tmem + L::P0 + wg * L::P_STEP + row, tO = tmem + L::O0 + wg * HD + row;
+      const uint32_t tO = tmem + L::O0 + wg * HD + row;
       uint8_t* q_at = sQ + wg * L::Q;
       uint32_t kv_it = 0, it = 0, turns = 0;                   // key tiles so far; those of this warpgroup; its turns at the exponentials
       bool ok = true;
-      TlWalk w = start;
+      TlWalk<L::AHEAD> w = start;
       while (w.f < w.end && ok) {
-        const TlItem item = tl_item(p, w.s, G, w.qt);
+        const TlItem item = tl_item<L::KEYS>(p, w.s, G, w.qt);
         const int rows = w.s.n * G, first = w.qt * TL_ROWS + wg * 128;
         int k0, k1;
         w.part(item, k0, k1);
@@ -248,14 +250,16 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           float m2 = -1e30f, l = 0.f;
           int E = -1000;
           for (int t = k0; t < k1; ++t, ++it, ++kv_it) {
-            if (!tl_wait(&s_full[wg], it & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
+            const uint32_t buf = L::BUFS == 2 ? it & 1u : 0u, phase = (L::BUFS == 2 ? it >> 1 : it) & 1u;
+            const uint32_t tS = tmem + wg * 128 + buf * 64 + row, tP = L::OVER ? tS : tmem + L::P0 + wg * 64 + row;
+            if (!tl_wait(&s_full[2 * wg + buf], phase, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
             tc_fence_after();
-            const float4 sc = scales[kv_it & 3];
-            float x[128];
+            const float4 sc = scales[kv_it & 7];
+            float x[L::KEYS];
             {
               uint32_t(*rg)[32] = reinterpret_cast<uint32_t(*)[32]>(x);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, rg[c]);
+              for (int c = 0; c < L::KEYS / 32; ++c) tmem_ld_32x32(tS + c * 32, rg[c]);
               tmem_ld_wait();
             }
             if constexpr (!L::OVER) {                          // the next scores may come
@@ -263,12 +267,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
               __syncwarp();
               if (lane == 0) mbar_arrive(&s_free[wg]);
             }
-            const int base = (item.lo + t) * TL_KEYS;
-            if (base + TL_KEYS - 1 > pos_a || (p.window > 0 && pos_z - p.window + 1 > base) || sc.x < 0.f || sc.y < 0.f) {
+            const int base = (item.lo + t) * L::KEYS;
+            if (base + L::KEYS - 1 > pos_a || (p.window > 0 && pos_z - p.window + 1 > base) || sc.x < 0.f || (L::PP > 1 && sc.y < 0.f)) {
               // a bit a column, so that a column costs a test and a choice: three comparisons each were a third of the loop's code, and its fetching showed
               const int hi = pos - base, lo = p.window > 0 ? pos - p.window + 1 - base : 0;
 #pragma unroll
-              for (int w = 0; w < 4; ++w) {
+              for (int w = 0; w < L::KEYS / 32; ++w) {
                 const int h = hi - 32 * w, l0 = lo - 32 * w;              // columns l0 ... h of this word
                 uint32_t see = (h >= 31 ? 0xffffffffu : h < 0 ? 0u : (2u << h) - 1u) & (l0 <= 0 ? 0xffffffffu : l0 > 31 ? 0u : 0xffffffffu << l0);
                 if ((w < 2 ? sc.x : sc.y) < 0.f) see = 0u;
@@ -281,9 +285,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             float f[2] = {qs * fabsf(sc.x), qs * fabsf(sc.y)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) f[h] = f[h] == 0.f ? 1e-37f : f[h];
-            float mt[2];
+            float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < L::PP; ++h) {
               float mr[4];
 #pragma unroll
               for (int c = 0; c < 4; ++c) mr[c] = fmaxf(x[h * 64 + c], x[h * 64 + 4 + c]);
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
               mt[h] = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3])) * f[h];
             }
             const float top = fmaxf(mt[0], mt[1]);
-            const int e0 = (int)(__float_as_uint(sc.z) >> 23) - 127, e1 = (int)(__float_as_uint(sc.w) >> 23) - 127, En = max(E, max(e0, e1));
+            const int e0 = (int)(__float_as_uint(sc.z) >> 23) - 127, e1 = L::PP > 1 ? (int)(__float_as_uint(sc.w) >> 23) - 127 : e0, En = max(E, max(e0, e1));
             // the last second product is done: its weights' places are free, its sums can be rescaled
             const bool grow = __any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E);
             if (t > k0 && (!L::OVER || grow)) {
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             }
             const float de[2] = {fmaxf((float)(e0 - En), -60.f), fmaxf((float)(e1 - En), -60.f)};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < L::PP; ++h) {
               const float2 ff = make_float2(f[h], f[h]), bias = make_float2(TL_OFF + de[h] - m2, TL_OFF + de[h] - m2);
               float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -349,13 +353,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[wg]);
+            if (lane == 0) mbar_arrive(&p_ready[2 * wg + buf]);
           }
           if (!ok) break;
           if (!tl_wait(&o_full[wg], (it - 1u) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const bool whole = k0 == 0 && k1 == item.n;
-          const int f0 = w.f - w.k + TL_AHEAD, slot = 2 * blockIdx.x + (f0 > start.f ? 1 : 0);
+          const int f0 = w.f - w.k + L::AHEAD, slot = 2 * blockIdx.x + (f0 > start.f ? 1 : 0);
           float* rec = records + (size_t)slot * L::REC;
           const float fac = l == 0.f ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23) / l;
           T* dst = reinterpret_cast<T*>(p.out) + (long long)(w.s.first + i) * p.ld_o + (long long)(w.g * G + rr - i * G) * HD;
@@ -392,22 +396,22 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_E));
       // ------------------------------------------------------------------------------------------ pages to float16
       const int tid = threadIdx.x - 256;
-      constexpr int NK = HD / 16;                              // chunks of 16 codes a thread has of a tile's keys, and of its values
+      constexpr int NK = HD * L::KEYS / 2048, NP = NK / L::PP;                            // chunks of 16 codes a thread has of a tile's keys, and of its values
       uint32_t kv_it = 0;
       bool ok = true;
-      TlWalk w = start;
+      TlWalk<L::AHEAD> w = start;
       while (w.f < w.end && ok) {
-        const TlItem item = tl_item(p, w.s, G, w.qt);
+        const TlItem item = tl_item<L::KEYS>(p, w.s, G, w.qt);
         const int last = (w.s.start + w.s.n - 1) / PG;
         int k0, k1;
         w.part(item, k0, k1);
         uint4 rk[NK], rv[NK];
-        int id[2], after[2];                                   // pages of the tile whose codes are on their way; what the table has for the one behind it
+        int id[L::PP], after[L::PP];                                   // pages of the tile whose codes are on their way; what the table has for the one behind it
         float sc = 0.f;
         auto look = [&](int t) {                               // nothing waits for the answer here
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int pg = 2 * (item.lo + t) + h;
+          for (int h = 0; h < L::PP; ++h) {
+            const int pg = L::PP * (item.lo + t) + h;
             after[h] = t < k1 && pg <= last ? a.table[(long long)w.b * a.W + pg] : -2;
           }
         };
@@ -415,23 +419,23 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
         auto fetch = [&](uint4 (&r)[NK], const signed char* from) {
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
-            const int h = c / (NK / 2), ch = (c % (NK / 2)) * 128 + tid;
+            const int h = c / NP, ch = (c % NP) * 128 + tid;
             const long long at = ((long long)max(id[h], 0) * a.KV + w.g) * (PG * HD);
             r[c] = id[h] < 0 ? make_uint4(0, 0, 0, 0) : reinterpret_cast<const uint4*>(from + at)[ch];
           }
         };
         auto fetch_keys = [&](int t) {                         // and the scales of tile t, the pages' numbers of tile t + 1
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < L::PP; ++h) {
             id[h] = after[h];
             if ((unsigned)id[h] >= (unsigned)a.pages) {
-              if (id[h] != -2 || 2 * (item.lo + t) + h <= last) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
+              if (id[h] != -2 || L::PP * (item.lo + t) + h <= last) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
               id[h] = -1;
             }
           }
           fetch(rk, a.k);
           if (tid < 4) {
-            const int page = tid & 1 ? id[1] : id[0];
+            const int page = id[L::PP > 1 ? tid & 1 : 0];
             sc = page >= 0 ? (tid < 2 ? a.ks : a.vs)[(long long)page * a.KV + w.g] : tid < 2 ? -1.f : PG_LEAST;
           }
           look(t + 1);
@@ -448,17 +452,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           if (!tl_wait(&k_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
-            const int ch = (c % (NK / 2)) * 128 + tid, key = c / (NK / 2) * 64 + ch / (HD / 16), d = (ch % (HD / 16)) * 16;      // 16 dimensions of a key
+            const int ch = (c % NP) * 128 + tid, key = c / NP * 64 + ch / (HD / 16), d = (ch % (HD / 16)) * 16;      // 16 dimensions of a key
             uint32_t x[8];
             pg_halves(rk[c].x, x[0], x[1]);
             pg_halves(rk[c].y, x[2], x[3]);
             pg_halves(rk[c].z, x[4], x[5]);
             pg_halves(rk[c].w, x[6], x[7]);
-            uint8_t* kp = sk + (d >> 6) * (128 * 128);
+            uint8_t* kp = sk + (d >> 6) * (L::KEYS * 128);
             *reinterpret_cast<uint4*>(kp + sw128_off(key, d & 63)) = make_uint4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<uint4*>(kp + sw128_off(key, (d & 63) + 8)) = make_uint4(x[4], x[5], x[6], x[7]);
           }
-          if (tid < 4) reinterpret_cast<float*>(&scales[kv_it & 3])[tid] = sc;
+          if (tid < 4) reinterpret_cast<float*>(&scales[kv_it & 7])[tid] = sc;
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&k_full[st]);
@@ -466,13 +470,13 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           if (!tl_wait(&v_empty[st], free, a.status, ST_TIMEOUT_EMPTY, abort_flag)) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
-            const int ch = (c % (NK / 2)) * 128 + tid, vd = ch >> 2, vt = (ch & 3) * 16;                                          // 16 tokens of a dimension
+            const int ch = (c % NP) * 128 + tid, vd = ch >> 2, vt = (ch & 3) * 16;                                          // 16 tokens of a dimension
             uint32_t x[8];
             pg_halves(rv[c].x, x[0], x[1]);
             pg_halves(rv[c].y, x[2], x[3]);
             pg_halves(rv[c].z, x[4], x[5]);
             pg_halves(rv[c].w, x[6], x[7]);
-            uint8_t* vp = sv + c / (NK / 2) * (HD * 128);
+            uint8_t* vp = sv + c / NP * (HD * 128);
             *reinterpret_cast<uint4*>(vp + sw128_off(vd, vt)) = make_uint4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<uint4*>(vp + sw128_off(vd, vt + 8)) = make_uint4(x[4], x[5], x[6], x[7]);
           }
@@ -486,64 +490,87 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       }
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_I));
-      if (warp == 12) {
+      if (warp < 14) {
       // ------------------------------------------------------------------------------------------ MMAs
       const uint32_t on = elect_one();
-      const uint32_t id_s = make_idesc_f16(0, 0, 0, 128, TL_KEYS), id_o = make_idesc_f16(0, 0, 0, 128, HD);
-      uint32_t kv_it = 0, q_it[2] = {0, 0}, it[2] = {0, 0};
-      TlWalk w = start;
+      const uint32_t id_s = make_idesc_f16(0, 0, 0, 128, L::KEYS), id_o = make_idesc_f16(0, 0, 0, 128, HD);
+      // What the loops go by is handed around by lane 0, which is how the compiler learns that it is the same for all: counters, descriptors and addresses then stay in
+      // uniform registers, where these instructions want them (descriptors found lane by lane made issuing a tile's products take 1400 cycles a warpgroup).
+      const int wg = warp - 12;
+      uint32_t kv_it = 0, q_it = 0, it = 0, s_it = 0;          // key tiles; this warpgroup's pieces, tiles summed, tiles scored
+      TlWalk<L::AHEAD> w = start;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), tS = tm + __shfl_sync(0xffffffffu, wg, 0) * 128;
+      const uint32_t tO = tm + L::O0 + __shfl_sync(0xffffffffu, wg, 0) * HD, tP = L::OVER ? tS : tm + L::P0 + __shfl_sync(0xffffffffu, wg, 0) * 64;
+      const uint64_t dq = make_smem_desc_sw128(smem_u32(sQ) + __shfl_sync(0xffffffffu, wg, 0) * L::Q, 16, 1024), dkv = make_smem_desc_sw128(smem_u32(sKV), 16, 1024);
       auto full = [&](uint64_t* bar, uint32_t at) {
         wait_or_report(&bar[at % L::STAGES], (at / L::STAGES) & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
         tc_fence_after();
       };
-      while (w.f < w.end) {
-        const TlItem item = tl_item(p, w.s, G, w.qt);
+      bool more = w.f < w.end;
+      while (__shfl_sync(0xffffffffu, (int)more, 0)) {
+        const TlItem item = tl_item<L::KEYS>(p, w.s, G, w.qt);
         int k0, k1;
         w.part(item, k0, k1);
-        const int groups = w.qt * TL_ROWS + 128 < w.s.n * G ? 2 : 1;
-        auto scores = [&](int wg, uint32_t at) {
-          mma_kmajor_kmajor<HD>(on, tmem + wg * 128, smem_u32(sQ + wg * L::Q), smem_u32(sKV + (at % L::STAGES) * L::STAGE), id_s, false);
-          if (on) mbar_arrive(&s_full[wg]);                    // hands on what k_full brought: the scales, which no MMA touches
-          umma_commit_on(on, &s_full[wg]);
-          if (wg == groups - 1) umma_commit_on(on, &k_empty[at % L::STAGES]);
-        };
-        if (k0 < k1) {
-          full(k_full, kv_it);
-          for (int wg = 0; wg < groups; ++wg) {
-            wait_or_report(&q_full[wg], q_it[wg] & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
-            ++q_it[wg];
-            tc_fence_after();
-            scores(wg, kv_it);
-          }
-        }
-        for (int t = k0; t < k1; ++t, ++kv_it) {
-          if (!L::OVER) {
-            if (t + 1 < k1) full(k_full, kv_it + 1);
-            for (int wg = 0; wg < groups; ++wg) {
-              wait_or_report(&s_free[wg], it[wg] & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
-              tc_fence_after();
-              if (t + 1 < k1) scores(wg, kv_it + 1);
-            }
-          }
-          full(v_full, kv_it);
-          const uint32_t sv = smem_u32(sKV + (kv_it % L::STAGES) * L::STAGE + L::K);
-          for (int wg = 0; wg < groups; ++wg) {
-            wait_or_report(&p_ready[wg], it[wg] & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
-            ++it[wg];
-            tc_fence_after();
+        const bool two = __shfl_sync(0xffffffffu, (int)(w.qt * TL_ROWS + 128 < w.s.n * G), 0) != 0;
+        const int all = __shfl_sync(0xffffffffu, k1 - k0, 0), n = wg == 1 && !two ? 0 : all;
+        auto scores = [&](uint32_t at) {
+          const uint32_t buf = L::BUFS == 2 ? s_it & 1u : 0u;
+          ++s_it;
+          const uint64_t db = dkv + (at % L::STAGES) * (L::STAGE >> 4);
 #pragma unroll
-            for (int kk = 0; kk < TL_KEYS / 16; ++kk)
-              umma_f16_ts_on(on, tmem + L::O0 + wg * HD, tmem + L::P0 + wg * L::P_STEP + kk * 8,
-                             make_smem_desc_sw128(sv + (kk >> 2) * (HD * 128) + (kk & 3) * 32, 16, 1024), id_o, t > k0 || kk > 0 ? 1u : 0u);
-            umma_commit_on(on, &o_full[wg]);
-            if (wg == groups - 1) umma_commit_on(on, &v_empty[kv_it % L::STAGES]);
-            if (L::OVER && t + 1 < k1) {
-              full(k_full, kv_it + 1);
-              scores(wg, kv_it + 1);
-            }
+          for (int kk = 0; kk < HD / 16; ++kk)
+            umma_f16_on(on, tS + buf * 64, dq + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4), db + (((kk >> 2) * (L::KEYS * 128) + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
+          if (on) mbar_arrive(&s_full[2 * wg + buf]);          // hands on what k_full brought: the scales, which no MMA touches
+          umma_commit_on(on, &s_full[2 * wg + buf]);
+          umma_commit_on(on, &k_empty[at % L::STAGES]);
+        };
+#pragma unroll
+        for (int j = 0; j < L::BUFS; ++j) {
+          if (j >= n) continue;
+          full(k_full, kv_it + j);
+          if (j == 0) {
+            wait_or_report(&q_full[wg], q_it & 1u, a.status, ST_TIMEOUT_FULL, abort_flag);
+            ++q_it;
+            tc_fence_after();
           }
+          scores(kv_it + j);
         }
+        for (int t = 0; t < n; ++t) {
+          const uint32_t at = kv_it + t, buf = L::BUFS == 2 ? it & 1u : 0u, phase = (L::BUFS == 2 ? it >> 1 : it) & 1u;
+          if (!L::OVER && t + 1 < n) {
+            full(k_full, at + 1);
+            wait_or_report(&s_free[wg], it & 1u, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
+            tc_fence_after();
+            scores(at + 1);
+          }
+          full(v_full, at);
+          const uint64_t dv = dkv + (((at % L::STAGES) * L::STAGE + L::K) >> 4);
+          wait_or_report(&p_ready[2 * wg + buf], phase, a.status, ST_TIMEOUT_TMEM_EMPTY, abort_flag);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < L::KEYS / 16; ++kk)
+            umma_f16_ts_on(on, tO, tP + buf * 64 + kk * 8, dv + (((kk >> 2) * (HD * 128) + (kk & 3) * 32) >> 4), id_o, t > 0 || kk > 0 ? 1u : 0u);
+          umma_commit_on(on, &o_full[wg]);
+          umma_commit_on(on, &v_empty[at % L::STAGES]);
+          if (L::OVER && t + L::BUFS < n) {
+            // scores go where these weights are, and products of different accumulators need not run in the order of their issue
+            full(k_full, at + L::BUFS);
+            wait_or_report(&o_full[wg], it & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag);
+            tc_fence_after();
+            scores(at + L::BUFS);
+          }
+          ++it;
+        }
+        // Tiles that are the other warpgroup's alone are followed stage by stage all the same: a barrier's phase is known by its parity, so neither warp may be more than one ahead.
+        for (int t = n; t < all; ++t) {
+          full(k_full, kv_it + t);
+          if (on) mbar_arrive(&k_empty[(kv_it + t) % L::STAGES]);
+          full(v_full, kv_it + t);
+          if (on) mbar_arrive(&v_empty[(kv_it + t) % L::STAGES]);
+        }
+        kv_it += all;
         w.next(p, G, cum, item);
+        more = w.f < w.end;
       }
       __syncwarp();
       }
@@ -603,7 +630,7 @@ template <typename T, int HD>
 static int tl_go(const PgAttn& p, cudaStream_t st) {
   using L = Tl<HD>;
   // at least 120 KB, so that one block takes an SM with its tensor memory
-  const size_t smem = std::max<size_t>(120 * 1024, 1024 + 2 * L::Q + L::STAGES * (L::STAGE + 32) + 16 * 8 + 64 + 16 + (size_t)(p.a.B + 1) * 4);
+  const size_t smem = std::max<size_t>(120 * 1024, 1024 + 2 * L::Q + L::STAGES * (L::STAGE + 32) + 16 * 8 + 128 + 16 + (size_t)(p.a.B + 1) * 4);
   const int blocks = pg_sms();
   GB_PDL_LAUNCH_SMEM((paged_tile_kernel<T, HD>), dim3(blocks), dim3(TL_THREADS), smem, st, p);
   const int rc = gb_launch_rc();

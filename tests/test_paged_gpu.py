@@ -281,6 +281,15 @@ def test_prompts(hd, H, KV, dt, window):
     run_attn(P, L, hd, H, KV, dt, [0, 100, 1, 191, 640], [129, 64, 0, 257, 1], window)
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_items_of_half_and_whole_tiles_take_turns(hd):
+    """Rows of a key head that end in the first or the second 128 of 256, over many key tiles: what one half of a block leaves out the other half's warps must not run ahead of."""
+    P, L = ops()
+    run_attn(P, L, hd, 6, 2, "f16", [3000, 2000, 700], [90, 171, 43], 0)
+    run_attn(P, L, hd, 6, 2, "bf16", [1900, 5, 4000], [30, 300, 86], 1500)
+    run_attn(P, L, hd, 8, 8, "f16", [1000, 1200], [257, 385], 0)
+
+
 def test_long_sequences_are_split_and_joined():
     P, L = ops()
     run_attn(P, L, 64, 4, 2, "f16", [20001, 3, 9000], [1, 1, 1], 0)
