@@ -52,7 +52,10 @@ __device__ __forceinline__ TkPages tk_pages(const PgAttn& p, const PgSeq& s) {
 }
 
 // Whose piece a warp left in a record: the item, its places, its sequence's first row, its rows.
-struct TkCut { int item, f0, f1, first, rows; };
+struct TkCut { int item, f0, f1, first, rows, quota, pad0, pad1; };
+// In the workspace: two of these a block, item -1 where there is nothing, then the records of which blocks' pieces they are.
+__device__ __forceinline__ TkCut* tk_cuts(const PgAttn& p) { return reinterpret_cast<TkCut*>(p.part); }
+__device__ __forceinline__ float* tk_parts(const PgAttn& p, int blocks) { return p.part + (size_t)2 * blocks * (sizeof(TkCut) / 4); }
 // A record: R x HD results, then R pairs (maximum, sum)
 template <int HD> __host__ __device__ constexpr int tk_record(int R) { return R * (HD + 2); }
 
@@ -122,6 +125,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
     if (threadIdx.x == 0) cum[0] = 0;
     __syncthreads();
   }
+  if (!item_mode && threadIdx.x == 0) tk_cuts(p)[2 * blockIdx.x].item = tk_cuts(p)[2 * blockIdx.x + 1].item = -1;
   const int total = KVs * cum[nb];
   const int blocks = item_mode ? 1 : (int)gridDim.x, quota = max(1, (total + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
   const int c_lo = item_mode ? 0 : min(total, (int)blockIdx.x * TK_WARPS * quota), c_hi = min(total, c_lo + TK_WARPS * quota);
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         }
       }
     }
-    if (!whole && lane == 0) cut[2 * warp + (first ? 0 : 1)] = {item, f_begin, f_end, sq.first, rows};
+    if (!whole && lane == 0) cut[2 * warp + (first ? 0 : 1)] = {item, f_begin, f_end, sq.first, rows, quota, 0, 0};
     __syncwarp();
   };
 
@@ -439,18 +443,22 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
     const TkCut c = cut[k0];
     const bool whole = c.f0 >= c_lo && c.f1 <= c_hi;
     const int g = g_base + c.item % KVs;
-    float* part = p.part + (size_t)(2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0)) * rec_n;
+    float* part = tk_parts(p, blocks) + (size_t)(2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0)) * rec_n;
+    // an item's records: perhaps the last one of a warp (odd), then first ones of the warps behind it
+    const int w0 = (k0 + 1) >> 1, w1 = (k1 + 1) >> 1;
     for (int i = threadIdx.x; i < c.rows * (HD / 2); i += TK_THREADS) {
       const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
       float sum = 0.f, u = 0.f, v = 0.f;
-#pragma unroll 4
-      for (int k = k0; k < k1; ++k) {                                 // records of nobody weigh nothing, whatever they hold
-        const float w = wt[k * R + r];
-        const float2 x = *reinterpret_cast<const float2*>(rec_of(k) + r * HD + d);
+      auto add = [&](float w, const float* rec) {                     // what weighs nothing adds nothing, whatever it holds
+        const float2 x = *reinterpret_cast<const float2*>(rec);
         sum += w;
         u += w == 0.f ? 0.f : w * x.x;
         v += w == 0.f ? 0.f : w * x.y;
-      }
+      };
+      if (k0 & 1) add(wt[k0 * R + r], rec_of(k0) + r * HD + d);
+      const float *rec = heads + w0 * rec_n + r * HD + d, *wr = wt + 2 * w0 * R + r;
+#pragma unroll 4
+      for (int w = w0; w < w1; ++w, rec += rec_n, wr += 2 * R) add(*wr, rec);
       const float f = sum == 0.f ? 0.f : __fdividef(1.f, sum);
       if (whole) {
         *reinterpret_cast<uint32_t*>(tk_out<T, HD>(p, c.first, g, r) + d) = Cvt<T>::pack2(u * f, v * f);
@@ -463,53 +471,44 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         }
       }
     }
+    if (!whole && threadIdx.x == 0) tk_cuts(p)[2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0)] = c;
   }
 }
 
-// Joins what blocks left of an item: one block a (row, key head, sequence).
+// Joins what blocks left of the item that begins in block x's run and is cut by its end: one block a row.
 constexpr int TJ_THREADS = 128;
 template <typename T, int HD>
 __global__ void __launch_bounds__(TJ_THREADS) paged_join_kernel(const __grid_constant__ PgAttn p, int R, int blocks) {
-  __shared__ int red[2][4];
   __shared__ float top_of[4], wt[PG_MOST_BLOCKS], sums[TJ_THREADS / 32], acc_of[TJ_THREADS];
-  const gb_paged& a = p.a;
-  const int r = blockIdx.x, g = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // starts and counts are older than the launch ahead, which is past its own wait: only its records are waited for
-  int before = 0, all = 0;
-  for (int i = threadIdx.x; i < a.B; i += TJ_THREADS) {
-    const int n = tk_pages(p, pg_seq(a, i)).n;
-    all += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if (lane == 0) { red[0][warp] = before; red[1][warp] = all; }
-  const PgSeq s = pg_seq(a, b);
-  __syncthreads();
-  before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-  const int total = a.KV * (red[1][0] + red[1][1] + red[1][2] + red[1][3]);
-  const int np = tk_pages(p, s).n, G = p.H / a.KV;
-  const int span = TK_WARPS * max(1, (total + TK_WARPS * blocks - 1) / (TK_WARPS * blocks));
-  const int f0 = a.KV * before + g * np, c0 = f0 / span, c1 = (f0 + np - 1) / span;
-  const bool mine = np > 0 && r < s.n * G && c0 != c1;       // else one block had all of it
+  const int c0 = blockIdx.x, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  if (!mine) return;
-  const int rec_n = tk_record<HD>(R), n = c1 - c0 + 1;
-  auto rec_of = [&](int c) { return p.part + (size_t)(2 * c + (f0 > c * span ? 1 : 0)) * rec_n; };
+  // of the two, the later begins last
+  const TkCut a0 = tk_cuts(p)[2 * c0], a1 = tk_cuts(p)[2 * c0 + 1];
+  const int k = a1.item >= 0 ? 1 : 0;
+  const TkCut c = k ? a1 : a0;
+  const int span = TK_WARPS * c.quota;
+  if (c.item < 0 || r >= c.rows || c.f0 < c0 * span || c.f1 <= (c0 + 1) * span) return;
+  const int rec_n = tk_record<HD>(R), n = (c.f1 - 1) / span - c0 + 1;
+  const float* parts = tk_parts(p, blocks);
+  auto rec_of = [&](int j) { return parts + (size_t)(j == 0 ? 2 * c0 + k : 2 * (c0 + j)) * rec_n; };
+  float2 ml[PG_MOST_BLOCKS / TJ_THREADS];
   float top = -1e30f;
-  for (int c = threadIdx.x; c < n; c += TJ_THREADS) top = fmaxf(top, rec_of(c0 + c)[R * HD + 2 * r]);
+#pragma unroll
+  for (int i = 0; i < PG_MOST_BLOCKS / TJ_THREADS; ++i) {
+    const int j = i * TJ_THREADS + threadIdx.x;
+    ml[i] = j < n ? *reinterpret_cast<const float2*>(rec_of(j) + R * HD + 2 * r) : make_float2(-1e30f, 0.f);
+    top = fmaxf(top, ml[i].x);
+  }
   top = warp_max(top);
   if (lane == 0) top_of[warp] = top;
   __syncthreads();
   top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
   float sum = 0.f;
-  for (int c = threadIdx.x; c < n; c += TJ_THREADS) {
-    const float2 ml = *reinterpret_cast<const float2*>(rec_of(c0 + c) + R * HD + 2 * r);
-    wt[c] = ml.y == 0.f ? 0.f : ml.y * pg_ex2(ml.x - top);
-    sum += wt[c];
+#pragma unroll
+  for (int i = 0; i < PG_MOST_BLOCKS / TJ_THREADS; ++i) {
+    const float w = ml[i].y == 0.f ? 0.f : ml[i].y * pg_ex2(ml[i].x - top);
+    wt[i * TJ_THREADS + threadIdx.x] = w;
+    sum += w;
   }
   sum = warp_sum(sum);
   if (lane == 0) sums[warp] = sum;
@@ -518,13 +517,13 @@ __global__ void __launch_bounds__(TJ_THREADS) paged_join_kernel(const __grid_con
   const int d = threadIdx.x % HD;
   float acc = 0.f;
 #pragma unroll 8
-  for (int c = threadIdx.x / HD; c < n; c += TJ_THREADS / HD) acc = fmaf(wt[c], rec_of(c0 + c)[r * HD + d], acc);
+  for (int j = threadIdx.x / HD; j < n; j += TJ_THREADS / HD) acc = fmaf(wt[j], rec_of(j)[r * HD + d], acc);
   acc_of[threadIdx.x] = acc;
   __syncthreads();
   if (threadIdx.x < HD) {
 #pragma unroll
     for (int j = 1; j < TJ_THREADS / HD; ++j) acc += acc_of[threadIdx.x + j * HD];
-    tk_out<T, HD>(p, s.first, g, r)[d] = Cvt<T>::from_f(sum == 0.f ? 0.f : acc / sum);
+    tk_out<T, HD>(p, c.first, c.item % p.a.KV, r)[d] = Cvt<T>::from_f(sum == 0.f ? 0.f : acc / sum);
   }
 }
 
@@ -549,7 +548,7 @@ static int tk_go(const PgAttn& p, int R, cudaStream_t st) {
   GB_PDL_LAUNCH_SMEM((paged_token_kernel<T, HD, NQ>), dim3(blocks), dim3(TK_THREADS), smem, st, p, R, slots, item);
   const int rc = gb_launch_rc();
   if (rc || item) return rc;
-  GB_PDL_LAUNCH((paged_join_kernel<T, HD>), dim3(R, p.a.KV, p.a.B), dim3(TJ_THREADS), st, p, R, blocks);
+  GB_PDL_LAUNCH((paged_join_kernel<T, HD>), dim3(blocks, R), dim3(TJ_THREADS), st, p, R, blocks);
   return gb_launch_rc();
 }
 
@@ -562,7 +561,7 @@ static int tk_size(const PgAttn& p, int R, cudaStream_t st) {
 
 long long pg_token_ws(const PgAttn& p) {
   const int R = (int)(p.a.max_new * (p.H / p.a.KV));
-  return tk_item_mode(p) ? 0 : 2ll * pg_sms() * R * (p.a.hd + 2);
+  return tk_item_mode(p) ? 0 : 2ll * pg_sms() * (R * (p.a.hd + 2) + (long long)(sizeof(TkCut) / 4));
 }
 
 int pg_token_attn(const PgAttn& p, cudaStream_t st) {
