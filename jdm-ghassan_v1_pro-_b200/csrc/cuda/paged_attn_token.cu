@@ -36,15 +36,17 @@ __device__ __forceinline__ void tk_bulk(void* dst, const void* src, uint32_t byt
                : "memory");
 }
 
-// Where row r of (the sequence with rows from `first` on, key head g) goes.
+// Row r of a key head's queries: token r / G, head r % G of its group.
+struct TkRow { int token, head; };
+// Where the row goes, for the sequence with rows from `first` on and key head g.
 template <typename T, int HD>
-__device__ __forceinline__ T* tk_out(const PgAttn& p, int first, int g, int r) {
-  const int G = p.H / p.a.KV, i = r / G;
-  return reinterpret_cast<T*>(p.out) + (long long)(first + i) * p.ld_o + (long long)(g * G + r - i * G) * HD;
+__device__ __forceinline__ T* tk_out(const PgAttn& p, int first, int g, const TkRow& r) {
+  return reinterpret_cast<T*>(p.out) + (long long)(first + r.token) * p.ld_o + (long long)(g * (p.H / p.a.KV) + r.head) * HD;
 }
 
 // Pages of sequence b that its queries see: from page `lo`, `n` of them.
 struct TkPages { int lo, n; };
+struct TkSeq { PgSeq s; int lo; };           // a sequence and its first visible page
 __device__ __forceinline__ TkPages tk_pages(const PgAttn& p, const PgSeq& s) {
   if (s.n == 0) return {0, 0};
   const int lo = p.window > 0 ? max(0, s.start - p.window + 1) / PG : 0;
@@ -74,9 +76,12 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   int* scan = reinterpret_cast<int*>(wt + 2 * TK_WARPS * 8 * NQ);                             // sums of the warps
   volatile int* abort_flag = scan + TK_WARPS;
   int* cum = scan + TK_WARPS + 1;                                                             // pages of the sequences before
-  int* lows = cum + (item_mode ? 1 : p.a.B) + 1;                                              // their first visible pages
+  TkRow* rows_of = reinterpret_cast<TkRow*>(cum + (item_mode ? 1 : p.a.B) + 1);
+  TkSeq* seqs = reinterpret_cast<TkSeq*>(rows_of + 8 * NQ);
   uint64_t* bar = bars + warp * slots;
 
+  const int G = p.H / a.KV;
+  if (warp == 1 && lane < 8 * NQ) rows_of[lane] = {lane / G, lane % G};
   if (lane == 0) {
     for (int s = 0; s < slots; ++s) mbar_init(&bar[s], 1);
     cut[2 * warp].item = cut[2 * warp + 1].item = -1;
@@ -90,9 +95,10 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   if (item_mode) {
     if (threadIdx.x == 0) {
       cum[0] = 0;
-      const TkPages v = tk_pages(p, pg_seq(a, b_base));
+      const PgSeq sq = pg_seq(a, b_base);
+      const TkPages v = tk_pages(p, sq);
       cum[1] = v.n;
-      lows[0] = v.lo;
+      seqs[0] = {sq, v.lo};
     }
     __syncthreads();
   } else {
@@ -101,9 +107,10 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
       const int b = b0 + (int)threadIdx.x;
       int v = 0;
       if (b < nb) {
-        const TkPages seen = tk_pages(p, pg_seq(a, b));
+        const PgSeq sq = pg_seq(a, b);
+        const TkPages seen = tk_pages(p, sq);
         v = seen.n;
-        lows[b] = seen.lo;
+        seqs[b] = {sq, seen.lo};
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -144,24 +151,33 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   int E = -1000, item = -1, pos0 = 0, n_new = 0, f_begin = 0, f_end = 0;
   PgSeq sq{0, 0, 0};
 
-  auto load_queries = [&](int b, int g) {
-    const int G = p.H / a.KV;
+  // A lane has HD / 4 numbers of its rows, where it has them of a key.  Those of the warp's first item are asked for ahead of all else.
+  uint4 raw[NQ][HD / 32];
+  auto fetch_queries = [&](const PgSeq& s, int g) {
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      const int r = 8 * q + gq, i = r / G;
-      const bool on = r < sq.n * G;
+      const TkRow r = rows_of[8 * q + gq];
+      const bool on = r.token < s.n;
+      const T* src = reinterpret_cast<const T*>(p.q) + (long long)(s.first + (on ? r.token : 0)) * p.ld_q + (long long)(g * G + r.head) * HD + tq * VW;
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k) raw[q][k] = on ? *reinterpret_cast<const uint4*>(src + (k * 8 / VW) * 64 + (k * 8) % VW) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto make_queries = [&]() {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
       float x[HD / 4];
       uint32_t top = 0;
-      const long long row = (long long)(sq.first + (on ? i : 0)) * p.ld_q + (long long)(g * G + (on ? r - i * G : 0)) * HD;
 #pragma unroll
-      for (int c = 0; c < HD / 4 / VW; ++c) {
+      for (int k = 0; k < HD / 32; ++k) {
+        const uint32_t w[4] = {raw[q][k].x, raw[q][k].y, raw[q][k].z, raw[q][k].w};
 #pragma unroll
-        for (int k = 0; k < VW; k += 8) pg_load8(reinterpret_cast<const T*>(p.q) + row + 64 * c + tq * VW + k, x + c * VW + k);
-      }
-#pragma unroll
-      for (int k = 0; k < HD / 4; ++k) {
-        if (!on) x[k] = 0.f;
-        top = max(top, __float_as_uint(fabsf(x[k])));
+        for (int e = 0; e < 4; ++e) {
+          const float2 v = Cvt<T>::unpack2(w[e]);
+          x[8 * k + 2 * e] = v.x;
+          x[8 * k + 2 * e + 1] = v.y;
+          top = max(top, max(__float_as_uint(fabsf(v.x)), __float_as_uint(fabsf(v.y))));
+        }
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -192,7 +208,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   // the piece at hand is over: to the output where it is the whole item, else into a record
   auto finish = [&]() {
     if (item < 0) return;
-    const int rows = sq.n * (p.H / a.KV);
+    const int rows = sq.n * G;
     const bool whole = f_begin >= w_lo && f_end <= w_hi, first = f_begin <= w_lo;
     float* rec = first ? heads + warp * rec_n : reinterpret_cast<float*>(ring);
     const float unit = E < -500 ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23);
@@ -208,7 +224,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         const int r = 8 * q + 2 * tq + c;
         if (r >= rows) continue;
         if (whole) {
-          T* dst = tk_out<T, HD>(p, sq.first, g_base + item % KVs, r) + gq;
+          T* dst = tk_out<T, HD>(p, sq.first, g_base + item % KVs, rows_of[r]) + gq;
 #pragma unroll
           for (int k = 0; k < KK; ++k) {
             dst[16 * k] = Cvt<T>::from_f(o[q][k][c] * f);
@@ -231,6 +247,10 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
 
   int slot_in = 0, slot_out = 0;
   uint32_t parity = 0;
+  if (w_lo < w_hi) {
+    const int b = seq_of(w_lo);
+    fetch_queries(seqs[b].s, g_base + (w_lo - cum[b] * KVs) / (cum[b + 1] - cum[b]));
+  }
   for (int base = w_lo; base < w_hi; base += 32) {
     const int cnt = min(32, w_hi - base);
     // lane i looks up page i of the batch
@@ -244,7 +264,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
       const int local = f - cum[u_b] * KVs;
       u_g = local / u_np;
       u_f = cum[u_b] * KVs + u_g * u_np;      // where its item begins
-      u_p = lows[u_b] + local - u_g * u_np;
+      u_p = seqs[u_b].lo + local - u_g * u_np;
       u_id = pg_page(a, b_base + u_b, u_p);
       u_bad = u_id < 0;
       if (u_bad) u_id = 0;
@@ -272,10 +292,11 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         item = it;
         f_begin = f0;
         f_end = f0 + __shfl_sync(0xffffffffu, u_np, i);
-        sq = pg_seq(a, b_base + ub);
+        sq = seqs[ub].s;
         pos0 = sq.start;
         n_new = sq.n;
-        load_queries(b_base + ub, g_base + ug);
+        if (base != w_lo || i != 0) fetch_queries(sq, g_base + ug);
+        make_queries();
       }
       const float ks = __shfl_sync(0xffffffffu, u_ks, i), vs = __shfl_sync(0xffffffffu, u_vs, i);
       const bool all_bad = (bad >> i) & 1u;
@@ -324,12 +345,11 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         f[q][1] = qs[q][1] * ks;
       }
       if (edge) {
-        const int G = p.H / a.KV;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const int pos = pos0 + (8 * q + 2 * tq + c) / G;
+            const int pos = pos0 + rows_of[8 * q + 2 * tq + c].token;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -461,7 +481,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
       for (int w = w0; w < w1; ++w, rec += rec_n, wr += 2 * R) add(*wr, rec);
       const float f = sum == 0.f ? 0.f : __fdividef(1.f, sum);
       if (whole) {
-        *reinterpret_cast<uint32_t*>(tk_out<T, HD>(p, c.first, g, r) + d) = Cvt<T>::pack2(u * f, v * f);
+        *reinterpret_cast<uint32_t*>(tk_out<T, HD>(p, c.first, g, rows_of[r]) + d) = Cvt<T>::pack2(u * f, v * f);
       } else {
         *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(u * f, v * f);
         if (d == 0) {
@@ -523,7 +543,8 @@ __global__ void __launch_bounds__(TJ_THREADS) paged_join_kernel(const __grid_con
   if (threadIdx.x < HD) {
 #pragma unroll
     for (int j = 1; j < TJ_THREADS / HD; ++j) acc += acc_of[threadIdx.x + j * HD];
-    tk_out<T, HD>(p, c.first, c.item % p.a.KV, r)[d] = Cvt<T>::from_f(sum == 0.f ? 0.f : acc / sum);
+    const int G = p.H / p.a.KV;
+    tk_out<T, HD>(p, c.first, c.item % p.a.KV, {r / G, r % G})[d] = Cvt<T>::from_f(sum == 0.f ? 0.f : acc / sum);
   }
 }
 
@@ -540,7 +561,7 @@ template <typename T, int HD, int NQ>
 static int tk_go(const PgAttn& p, int R, cudaStream_t st) {
   const int item = tk_item_mode(p), blocks = item ? p.a.B * p.a.KV : pg_sms();
   const size_t fixed = ((size_t)TK_WARPS * tk_record<HD>(R) * 4 + 15) / 16 * 16 + 2 * TK_WARPS * (sizeof(TkCut) + 8 * NQ * 4) +
-                       (TK_WARPS + 1 + 2 * (item ? 1 : p.a.B) + 1) * 4;
+                       (TK_WARPS + 1 + 5 * (item ? 1 : p.a.B) + 1 + 2 * 8 * NQ) * 4;
   constexpr int most = HD == 32 ? 8 : HD == 64 ? 5 : 3;
   const int slots = (int)std::min<size_t>(most, (TK_SMEM - fixed) / (TK_WARPS * ((size_t)PG * HD + 8)));
   if (slots < 2) return -3;
