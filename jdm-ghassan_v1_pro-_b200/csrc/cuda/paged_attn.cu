@@ -21,10 +21,16 @@ int pg_sms() {
 
 using namespace gb;
 
-// The sequences from b0 on, at most PG_MOST_SEQS of them.
+// Sequences of a launch: work is dealt by places counted in 32 bits, a sequence's being at most its pages or, for every 256 query rows, its key tiles and two more.
+static int gb_paged_most_seqs(const gb_paged* a, int H) {
+  const long long items = ((long long)a->max_new * (H / a->KV) + 255) / 256;
+  const double places = (double)a->KV * items * (a->W + 2);
+  return (int)std::min<double>(PG_MOST_SEQS, 2e9 / places);
+}
+// The sequences from b0 on, as many as fit.
 static PgAttn gb_paged_some(const PgAttn& p, int b0) {
   PgAttn s = p;
-  s.a.B = std::min(PG_MOST_SEQS, p.a.B - b0);
+  s.a.B = std::min(gb_paged_most_seqs(&p.a, p.H), p.a.B - b0);
   s.a.table += (long long)b0 * p.a.W;
   s.a.start += b0;
   if (s.a.count) {
@@ -41,9 +47,8 @@ static PgAttn gb_paged_some(const PgAttn& p, int b0) {
 static int gb_paged_attn_args(const gb_paged* a, int H, int window) {
   if (const int rc = gb_paged_check(a)) return rc;
   if (H <= 0 || H % a->KV || window < 0 || H > 65535) return -1;
-  // places that work is dealt by are counted in 32 bits: pages, or key tiles of every 256 rows
-  const long long items = ((long long)a->max_new * (H / a->KV) + 255) / 256, places = items > 1 ? items * ((a->W + 1) / 2 + 1) : a->W;
-  if ((long long)a->max_new * H > 0x7fffffffll || std::min(a->B, PG_MOST_SEQS) * (double)places * a->KV > 2e9) return -3;
+  if ((long long)a->max_new * H > 0x7fffffffll) return -3;
+  if (a->max_new > 0 && gb_paged_most_seqs(a, H) < 1) return -3;
   return 0;
 }
 
@@ -66,10 +71,11 @@ extern "C" int gb_paged_attn(const gb_paged* a, const void* q, long long ld_q, i
   if (need > 0 && (!ws || ws_floats < need || (reinterpret_cast<uintptr_t>(ws) & 15))) return -5;
   const PgAttn p = {*a, q, ld_q, H, scale * 1.4426950408889634f, window, out, ld_o, ws};
   const bool few = (long long)a->max_new * (H / a->KV) <= PG_TOKEN_ROWS;
-  for (int b0 = 0; b0 < a->B; b0 += PG_MOST_SEQS) {
+  for (int b0 = 0; b0 < a->B;) {
     const PgAttn s = gb_paged_some(p, b0);
     const int rc = few ? pg_token_attn(s, st) : pg_tile_attn(s, st);
     if (rc) return rc;
+    b0 += s.a.B;
   }
   return 0;
 }

@@ -6,7 +6,7 @@ namespace gb {
 
 constexpr int PG_TOKEN_ROWS = 16;            // query rows a key head (tokens x heads of a group) up to which the token kernel runs
 constexpr int PG_MOST_BLOCKS = 256;          // blocks that pieces are dealt to, at most
-constexpr int PG_MOST_SEQS = 2048;           // sequences of one launch; more are several launches
+constexpr int PG_MOST_SEQS = 1024;           // sequences of one launch (their numbers are in shared memory); more are several launches
 
 struct PgAttn {
   gb_paged a;

@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
       TlWalk<L::AHEAD> w = start;
       while (w.f < w.end && ok) {
         const TlItem item = tl_item<L::KEYS>(p, w.s, G, w.qt);
-        const int last = (w.s.start + w.s.n - 1) / PG;
+        // pages that the item's rows see: ahead of them there may be none any more (a window), although the first tile begins there
+        const int last = (w.s.start + w.s.n - 1) / PG, low = p.window > 0 ? max(0, w.s.start + w.qt * TL_ROWS / G - p.window + 1) / PG : 0;
         int k0, k1;
         w.part(item, k0, k1);
         uint4 rk[NK], rv[NK];
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
           for (int h = 0; h < L::PP; ++h) {
             const int pg = L::PP * (item.lo + t) + h;
-            after[h] = t < k1 && pg <= last ? a.table[(long long)w.b * a.W + pg] : -2;
+            after[h] = t < k1 && pg >= low && pg <= last ? a.table[(long long)w.b * a.W + pg] : -2;
           }
         };
         // codes of a tile's keys or values, chunk c of a page (HD * 64 codes) in the order of memory
@@ -429,7 +430,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) paged_tile_kernel(const __grid_
           for (int h = 0; h < L::PP; ++h) {
             id[h] = after[h];
             if ((unsigned)id[h] >= (unsigned)a.pages) {
-              if (id[h] != -2 || L::PP * (item.lo + t) + h <= last) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
+              const int pg = L::PP * (item.lo + t) + h;
+              if (pg >= low && pg <= last) atomicCAS(a.status, 0, ST_BAD_ARGUMENT);
               id[h] = -1;
             }
           }

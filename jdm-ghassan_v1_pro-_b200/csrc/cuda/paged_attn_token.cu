@@ -72,8 +72,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   float* heads = reinterpret_cast<float*>(smem + (size_t)TK_WARPS * slots * SLOT);            // records of the warps' first items
   uint64_t* bars = reinterpret_cast<uint64_t*>(heads + (TK_WARPS * rec_n + 1) / 2 * 2);
   TkCut* cut = reinterpret_cast<TkCut*>(bars + TK_WARPS * slots);                             // what the warps' records are of
-  float* wt = reinterpret_cast<float*>(cut + 2 * TK_WARPS);                                   // their weights, [record][row]
-  int* scan = reinterpret_cast<int*>(wt + 2 * TK_WARPS * 8 * NQ);                             // sums of the warps
+  int* scan = reinterpret_cast<int*>(cut + 2 * TK_WARPS);                                     // sums of the warps
   volatile int* abort_flag = scan + TK_WARPS;
   int* cum = scan + TK_WARPS + 1;                                                             // pages of the sequences before
   TkRow* rows_of = reinterpret_cast<TkRow*>(cum + (item_mode ? 1 : p.a.B) + 1);
@@ -433,65 +432,50 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   finish();
   __syncthreads();
 
-  // ---- pieces of the block's warps; those of one item are joined.  Loads are unconditional and picked from afterwards: behind branches each would wait for
-  // the one before (3400 cycles of the block's end, against 1000).
+  // ---- pieces of the block's warps; those of one item are joined, a warp a row.  A lane has a record's maximum and sum, so the weights need no shared memory and no further barrier
+  // (they took 1200 cycles of the block's end); loads are unconditional and picked from afterwards, since behind branches each would wait for the one before.
   auto rec_of = [&](int k) { return reinterpret_cast<const float*>((k & 1) ? smem + (size_t)(k >> 1) * slots * SLOT : reinterpret_cast<const uint8_t*>(heads + (k >> 1) * rec_n)); };
   constexpr int RECS = 2 * TK_WARPS;
-  {                                                                   // weight of record k in row r against the item's largest maximum
-    const int k = threadIdx.x % RECS, it = cut[k].item;
-    for (int r0 = 0; r0 < R; r0 += TK_THREADS / RECS) {               // as often for every lane: they exchange
-      const int r = min(r0 + (int)threadIdx.x / RECS, R - 1);
-      const float2 ml = *reinterpret_cast<const float2*>(rec_of(k) + R * HD + 2 * r);
-      float top = -1e30f;
-#pragma unroll
-      for (int j = 0; j < RECS; ++j) {
-        const float v = __shfl_sync(0xffffffffu, ml.x, j, RECS);
-        const int of = __shfl_sync(0xffffffffu, it, j, RECS);
-        top = fmaxf(top, of == it ? v : -1e30f);
-      }
-      wt[k * R + r] = it < 0 || ml.y == 0.f ? 0.f : ml.y * pg_ex2(ml.x - top);
-    }
-  }
-  __syncthreads();
   const int my_item = lane < RECS ? cut[lane].item : -1;
+  const float* my_rec = rec_of(min(lane, RECS - 1));
   unsigned left = __ballot_sync(0xffffffffu, my_item >= 0);
-  while (left) {
+  for (int turn = 0; left;) {
     const int k0 = __ffs(left) - 1;
     const unsigned same = __ballot_sync(0xffffffffu, my_item == __shfl_sync(0xffffffffu, my_item, k0));
-    const int k1 = 32 - __clz(same);
     left &= ~same;
     const TkCut c = cut[k0];
     const bool whole = c.f0 >= c_lo && c.f1 <= c_hi;
-    const int g = g_base + c.item % KVs;
-    float* part = tk_parts(p, blocks) + (size_t)(2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0)) * rec_n;
+    const int g = g_base + c.item % KVs, place = 2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0);
+    float* part = tk_parts(p, blocks) + (size_t)place * rec_n;
     // an item's records: perhaps the last one of a warp (odd), then first ones of the warps behind it
-    const int w0 = (k0 + 1) >> 1, w1 = (k1 + 1) >> 1;
-    for (int i = threadIdx.x; i < c.rows * (HD / 2); i += TK_THREADS) {
-      const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
-      float sum = 0.f, u = 0.f, v = 0.f;
-      auto add = [&](float w, const float* rec) {                     // what weighs nothing adds nothing, whatever it holds
-        const float2 x = *reinterpret_cast<const float2*>(rec);
-        sum += w;
-        u += w == 0.f ? 0.f : w * x.x;
-        v += w == 0.f ? 0.f : w * x.y;
-      };
-      if (k0 & 1) add(wt[k0 * R + r], rec_of(k0) + r * HD + d);
-      const float *rec = heads + w0 * rec_n + r * HD + d, *wr = wt + 2 * w0 * R + r;
-#pragma unroll 4
-      for (int w = w0; w < w1; ++w, rec += rec_n, wr += 2 * R) add(*wr, rec);
+    const int w0 = (k0 + 1) >> 1, w1 = (33 - __clz(same)) >> 1;
+    if (!whole && threadIdx.x == 0) tk_cuts(p)[place] = c;
+    for (int r = 0; r < c.rows; ++r, ++turn) {
+      if (turn % TK_WARPS != warp) continue;
+      const float2 at = *reinterpret_cast<const float2*>(my_rec + R * HD + 2 * r);
+      const bool mine = my_item == c.item;
+      const float top = warp_max(mine ? at.x : -1e30f);
+      const float weight = !mine || at.y == 0.f ? 0.f : at.y * pg_ex2(at.x - top), sum = warp_sum(weight);
       const float f = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-      if (whole) {
-        *reinterpret_cast<uint32_t*>(tk_out<T, HD>(p, c.first, g, rows_of[r]) + d) = Cvt<T>::pack2(u * f, v * f);
-      } else {
-        *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(u * f, v * f);
-        if (d == 0) {
-          float top = -1e30f;
-          for (int k = k0; k < k1; ++k) top = fmaxf(top, cut[k].item >= 0 ? rec_of(k)[R * HD + 2 * r] : -1e30f);
-          *reinterpret_cast<float2*>(part + R * HD + 2 * r) = make_float2(top, sum);
-        }
+#pragma unroll
+      for (int d0 = 0; d0 < HD; d0 += 64) {
+        const int d = d0 + 2 * lane % HD;                             // (hd 32: the upper lanes do the lower ones' work again)
+        float u = 0.f, v = 0.f;
+        auto add = [&](int k, const float* rec) {                     // what weighs nothing adds nothing, whatever it holds
+          const float w = __shfl_sync(0xffffffffu, weight, k);
+          const float2 x = *reinterpret_cast<const float2*>(rec);
+          u += w == 0.f ? 0.f : w * x.x;
+          v += w == 0.f ? 0.f : w * x.y;
+        };
+        if (k0 & 1) add(k0, rec_of(k0) + r * HD + d);
+        const float* rec = heads + w0 * rec_n + r * HD + d;
+#pragma unroll 4
+        for (int w = w0; w < w1; ++w, rec += rec_n) add(2 * w, rec);
+        if (whole) *reinterpret_cast<uint32_t*>(tk_out<T, HD>(p, c.first, g, rows_of[r]) + d) = Cvt<T>::pack2(u * f, v * f);
+        else *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(u * f, v * f);
       }
+      if (!whole && lane == 0) *reinterpret_cast<float2*>(part + R * HD + 2 * r) = make_float2(top, sum);
     }
-    if (!whole && threadIdx.x == 0) tk_cuts(p)[2 * blockIdx.x + (c.f0 > c_lo ? 1 : 0)] = c;
   }
 }
 
@@ -560,7 +544,7 @@ constexpr size_t TK_SMEM = 227 * 1024;
 template <typename T, int HD, int NQ>
 static int tk_go(const PgAttn& p, int R, cudaStream_t st) {
   const int item = tk_item_mode(p), blocks = item ? p.a.B * p.a.KV : pg_sms();
-  const size_t fixed = ((size_t)TK_WARPS * tk_record<HD>(R) * 4 + 15) / 16 * 16 + 2 * TK_WARPS * (sizeof(TkCut) + 8 * NQ * 4) +
+  const size_t fixed = ((size_t)TK_WARPS * tk_record<HD>(R) * 4 + 15) / 16 * 16 + 2 * TK_WARPS * sizeof(TkCut) +
                        (TK_WARPS + 1 + 5 * (item ? 1 : p.a.B) + 1 + 2 * 8 * NQ) * 4;
   constexpr int most = HD == 32 ? 8 : HD == 64 ? 5 : 3;
   const int slots = (int)std::min<size_t>(most, (TK_SMEM - fixed) / (TK_WARPS * ((size_t)PG * HD + 8)));

@@ -30,7 +30,8 @@ HEAD_DIMS = (32, 64, 128)
 
 
 class Pages(NamedTuple):
-    """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads]."""
+    """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads],
+    powers of two."""
     k: torch.Tensor
     ks: torch.Tensor
     v: torch.Tensor

@@ -304,6 +304,46 @@ def test_batches(B):
     run_attn(P, L, 64, 4, 2, "f16", [int(x) for x in r.integers(0, 260, B)], [1] * B, 0, gaps=False)
 
 
+@pytest.mark.parametrize("hd,n", [(32, 1), (128, 2), (32, 20)])
+def test_more_sequences_than_one_launch_takes(hd, n):
+    P, L = ops()
+    r = np.random.default_rng(n)
+    run_attn(P, L, hd, 8, 1, "f16", [int(x) for x in r.integers(0, 130, 1100)], [int(x) for x in r.integers(1, n + 1, 1100)], 0, gaps=False)
+
+
+def test_rows_without_first_and_count_are_one_a_sequence():
+    P, L = ops()
+    B, KV, hd, H = 1100, 1, 32, 2
+    seqs = seqs_of([1 + b % 70 for b in range(B)], KV, hd, 1)
+    pool = Pool(P, 2 * B, KV, hd)
+    table = pool.table([s.n for s in seqs])
+    for b, s in enumerate(seqs):
+        pool.fill(table, b, s)
+    start = [s.n - 1 for s in seqs]
+    q = torch.randn(B, H * hd, device="cuda").half()
+    out = P.attn(pool.p, q, table, i32(start), 1, H, 0.2)
+    k, v = P.read(pool.p, table, i32(start), 1, torch.float16, B)
+    L.check_status()
+    check_attn(out, q, seqs, start, [1] * B, list(range(B)), 0.2, 0, "f16", H, hd)
+    assert np.array_equal(v.double().cpu().numpy(), np.stack([s.held()[1][-1] for s in seqs]).astype(np.float16).astype(np.float64))
+
+
+@pytest.mark.parametrize("n,window", [(1, 100), (2, 64), (30, 70), (300, 129), (300, 1)])
+def test_pages_behind_the_window_may_be_gone(n, window):
+    """A text's pages that no query sees any more need not be in its table."""
+    P, L = ops()
+    KV, hd, H, start = 2, 64, 6, 900
+    seqs = seqs_of([start + n], KV, hd, 1)
+    pool = Pool(P, 30, KV, hd)
+    table = pool.table([start + n])
+    pool.fill(table, 0, seqs[0])
+    table[0, :(start - window + 1) // PAGE] = -1
+    q = torch.randn(n, H * hd, device="cuda").half()
+    out = P.attn(pool.p, q, table, i32([start]), n, H, 0.125, window=window, first=i32([0]), count=i32([n]))
+    L.check_status()
+    check_attn(out, q, seqs, [start], [n], [0], 0.125, window, "f16", H, hd)
+
+
 @pytest.mark.parametrize("n", [1, 30])
 def test_weights_far_apart_and_tiny_or_large_values(n):
     """One key that takes nearly all weight, and none; values of very small and large pages; queries at the ends of the type's range."""
