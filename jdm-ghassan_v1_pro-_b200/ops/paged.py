@@ -29,13 +29,16 @@ PAGE = 64
 HEAD_DIMS = (32, 64, 128)
 
 
-class Pages(NamedTuple):
-    """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads],
-    powers of two."""
+class _PoolTensors(NamedTuple):
     k: torch.Tensor
     ks: torch.Tensor
     v: torch.Tensor
     vs: torch.Tensor
+
+
+class Pages(_PoolTensors):
+    """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads],
+    powers of two.  The first call with a pool checks that they belong together."""
 
 
 class PagedArgs(ctypes.Structure):
@@ -83,6 +86,9 @@ def new_pages(pages: int, kv_heads: int, head_dim: int, device) -> Pages:
 
 def _pool(p: Pages, what):
     """(pages, kv_heads, head_dim, device index) of a pool whose tensors belong together."""
+    known = getattr(p, "_known", None)
+    if known is not None:
+        return known
     k, ks, v, vs = p
     if k.dim() == 4:
         pages, KV, page, hd = k.shape
@@ -91,7 +97,10 @@ def _pool(p: Pages, what):
                 and k.dtype is torch.int8 and v.dtype is torch.int8 and ks.dtype is torch.float32 and vs.dtype is torch.float32
                 and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
                 and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
-            return pages, KV, hd, dev
+            known = (pages, KV, hd, dev)
+            if isinstance(p, Pages):
+                p._known = known
+            return known
     raise ValueError(f"{what}: the pool's tensors do not belong together: contiguous int8 codes [pages, kv_heads, 64, head_dim] and [pages, kv_heads, head_dim, 64], float32 "
                      f"scales [pages, kv_heads], on one device; got " + ", ".join(f"{tuple(t.shape)} {t.dtype} on {t.device}" for t in p))
 
@@ -133,9 +142,9 @@ def _rows(t, width, dtype, dev, what):
 
 
 def _out(t, rows, width, like, dtype, dev, what):
-    """The tensor for ``rows`` rows of results and its row pitch."""
+    """The tensor for ``rows`` rows of results (of ``like``'s type) and its row pitch."""
     if t is None:
-        return like.new_empty((rows, width), dtype=dtype), width
+        return like.new_empty((rows, width)), width
     if t.shape[0] < rows:
         raise ValueError(f"{what}: {t.shape[0]} rows for the results of {rows}")
     return t, _rows(t, width, dtype, dev, what)
@@ -219,10 +228,21 @@ def read(pages: Pages, table, start, max_new: int, dtype, rows: int, *, first=No
     [rows, kv_heads * hd] tensors to write to."""
     pool = _pool(pages, "paged read")
     _, KV, hd, dev = pool
-    k, ld_k = _out(k_out, rows, KV * hd, pages.k, dtype, dev, "paged read")
-    v, ld_v = _out(v_out, rows, KV * hd, pages.k, dtype, dev, "paged read")
+    if rows < 0:
+        raise ValueError(f"paged read: {rows} rows")
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise ValueError(f"paged read: rows are float16 or bfloat16, not {dtype}")
+    if k_out is None or v_out is None:
+        k, v = pages.k.new_empty((2, rows, KV, hd), dtype=dtype).unbind(0)
+        at_k, at_v, ld_k, ld_v = k.data_ptr(), v.data_ptr(), KV * hd, KV * hd
+    if k_out is not None:
+        k_out, ld_k = _out(k_out, rows, KV * hd, None, dtype, dev, "paged read")
+        at_k, k = k_out.data_ptr(), k_out.unflatten(1, (KV, hd))
+    if v_out is not None:
+        v_out, ld_v = _out(v_out, rows, KV * hd, None, dtype, dev, "paged read")
+        at_v, v = v_out.data_ptr(), v_out.unflatten(1, (KV, hd))
     a = _args(pages, pool, table, start, max_new, first, count, rows, dtype, "paged read")
-    rc = _protos().gb_paged_read(a, k.data_ptr(), ld_k, v.data_ptr(), ld_v, _raw_stream(dev))
+    rc = _protos().gb_paged_read(a, at_k, ld_k, at_v, ld_v, _raw_stream(dev))
     if rc:
         _lib.check_rc(rc, "gb_paged_read")
-    return (k.view(rows, KV, hd) if k_out is None else k.unflatten(1, (KV, hd))), (v.view(rows, KV, hd) if v_out is None else v.unflatten(1, (KV, hd)))
+    return k, v
