@@ -2,7 +2,7 @@
 //
 // A page of a head is one block's: it sees all numbers that share a scale, and nobody else writes to the page, so nothing here needs an atomic or a second pass over
 // memory.  A page's rows of a query head are another block's, so that all of a block's loads are on their way before it waits for any: with the query heads in the loop of
-// their key head's block, a page at a time, six prompts of 7.7 thousand tokens (32/8 heads of 128) took twice as long.
+// their key head's block, a page at a time, appending six prompts of 7.7 thousand tokens (32/8 heads of 128) and reading them back took 76.9 us instead of 71.8.
 #include <algorithm>
 
 #include "paged_util.cuh"
@@ -33,12 +33,16 @@ __device__ __forceinline__ uint32_t pg_codes(const float* x, float inv) {
   return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
 }
 
-constexpr int PA_FEW = 64;                               // threads of a block with few new tokens a sequence: PA_FEW * 16 / HD at most
+// Threads of a block with few new tokens a sequence, PA_FEW * 16 / HD at most: more such blocks are on an SM.  us of appending and reading back, these blocks against 4 HD threads:
+// 12/4 heads of 64, 1 and 16 tokens, one sequence 4.0 and 4.1 against 4.4 and 5.1, 512 of them 14.7 and 22.2 against 26.4 and 42.3; 32/8 heads of 128, 1 and 8 tokens, 256
+// sequences 24.4 and 34.0 against 64.1 and 88.2.
+constexpr int PA_FEW = 64;
 
 // Blocks: (key head, behind them two query heads each; page of the new tokens; sequence): neighbours read neighbouring parts of the same rows.  HD / 16 lanes take a row:
 // each the 8 pairs 8c ... 8c + 7 that a rotation turns, as two vectors of 8 numbers.  4 HD threads have a page's 64 tokens at once, which 64 registers
 // allow; half the threads with two rows each took 114, two blocks an SM.  Bound by instructions issued as much as by memory: codes are rounded by an addition
-// and not by conversions, a page's values are turned in registers, four tokens to a word, not stored byte by byte.
+// and not by conversions, a page's values are turned in registers, four tokens to a word, not stored byte by byte.  Six prompts of 7.7 thousand tokens (32/8 heads of 128,
+// 98 MB read, 40 written): 39 us, memory 43 % and issue slots 53 % busy.
 template <typename T, int HD, int ROPE, int NT>
 __global__ void __launch_bounds__(NT, NT == PA_FEW ? 8 : 1024 / NT) paged_append_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ qkv, long long ld, int H,
                                                           T* __restrict__ q_out, long long ld_q, const float* __restrict__ qw,

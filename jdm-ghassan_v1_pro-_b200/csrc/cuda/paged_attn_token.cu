@@ -4,12 +4,14 @@
 // lengths are (mode "balanced"; the lengths are on the device and so is the dealing).  A warp streams its run through a ring of its own in shared memory, a bulk copy a
 // page of keys or values (4 KB at hd 64), and waits for nobody until its run is over: pieces of a (sequence, head) that lie in one warp are finished there, the others are joined
 // first in the block, then, across blocks, by a second kernel.  Where all items have a block each and few pages, a block takes an item and nothing is left to join (mode "item").
+// Whole calls: 192 sequences of 100 to 8000 tokens (8/2 heads of 64) 47.6 us, 4.2 TB/s of codes; one of 100001 (32/8 heads of 128) 44.2 us, 4.6 TB/s; 32 of 3 to 4095 (12/4 heads of
+// 64) 18.7 us, 1.9 TB/s, of which about 2.3 us pass before the first page is there and 3 us in joining a block's warps.
 //
 // A page is two products on the legacy tensor path, with the codes as float16 integers (exact): keys x queries and values x weights, so that
 // queries (8 columns) rather than keys are padded; 16 rows of queries would pad 3 of them to 16.  The order of the contracted dimensions is free as long as both operands have the
 // same, so a lane takes 16 consecutive bytes of a key, or of a value's tokens, and these are its MMA fragments.  The page's key scale joins the score's factor and its value
 // scale the exponent of the weights: w = 2^(s - m + 15 + e - E), with m the running maximum, e the value scale's exponent and E the largest so far.  Rounded to float16 a
-// weight is off by 2^-12 of itself, or by 2^-39 of the largest page's, whichever is more; the row sum has the unrounded weights.  Queries are scaled by a power of two so that a
+// weight is off by 2^-11 of itself, or by 2^-39 of the largest page's, whichever is more; the row sum has the unrounded weights.  Queries are scaled by a power of two so that a
 // row's largest is between 2^14 and 2^15: float16 then holds them as exactly as bfloat16 does.
 #include <algorithm>
 
@@ -18,7 +20,10 @@
 namespace gb {
 
 constexpr int TK_WARPS = 8, TK_THREADS = 32 * TK_WARPS;
-constexpr int TK_ITEM_PAGES = 16;            // most pages a sequence may show in mode "item"
+// Most pages a sequence may show in mode "item", which saves the second kernel and waits for a block's own pages only.  us, mode "item" against "balanced", 12/4 heads of 64, one
+// token behind 4, 8, 16, 24, 32 and 64 pages: one sequence 4.9, 5.4, 6.8, 8.3, 9.9, 16.1 against 7.0, 6.8, 8.2, 8.4, 8.6, 9.0; 32 sequences as long as each other gain more
+// (10.4 against 12.2 at 32 pages), but lengths are on the device and blocks of a ragged batch wait for the longest.
+constexpr int TK_ITEM_PAGES = 16;
 constexpr float TK_OFF = 15.f;               // weights are held as 2^15 of themselves, the most float16 takes
 
 __device__ __forceinline__ void tk_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
