@@ -7,7 +7,8 @@
 //
 // Every call names the sequences it works on in the same way: sequence b has start[b] tokens in the pages table[b][0 ...] before the call's own count[b] ones,
 // which are the rows first[b] ... first[b] + count[b] - 1 of the call's tensors (first NULL: row b; count NULL: one row each).  Rows that belong to no sequence are
-// neither read nor written.  What does not fit (more new tokens than max_new, positions past the table's width, rows outside the tensors, a negative number)
+// neither read nor written, and no row is two sequences'.  A page that a sequence appends to is in no other's table, nor twice in its own (pages that are only read may be), and
+// results do not lie over a call's inputs.  What does not fit (more new tokens than max_new, positions past the table's width, rows outside the tensors, a negative number)
 // leaves the sequence out, a page number outside the pool leaves the page's tokens out; both set the status to 301.
 #pragma once
 #include <cuda_runtime.h>

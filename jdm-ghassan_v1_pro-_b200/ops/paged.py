@@ -9,6 +9,7 @@ pages of one text may be anywhere in the pool, and one table serves all layers o
     q = paged.append(pages, qkv, table, start, max_new, cos_sin, H)        # rotate; keys and values into the pages
     o = paged.attn(pages, q, table, start, max_new, H, scale)              # the same table and start: attention up to each token's own place
 
+A page that one sequence appends to is in no other's table, nor twice in its own, and results do not lie over a call's inputs.
 Keys and values that are not finite are held as zero.  That, and numbers that do not fit (a page outside the pool, tokens past the table),
 set the device's status word, which ``_lib.check_status`` reads.
 """
@@ -38,7 +39,10 @@ class _PoolTensors(NamedTuple):
 
 class Pages(_PoolTensors):
     """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads],
-    powers of two.  The first call with a pool checks that they belong together."""
+    powers of two.  A call checks that they belong together, unless they are where they were when an earlier one did."""
+
+    def __reduce__(self):                                     # copies and what is loaded from a file are checked anew
+        return Pages, tuple(self)
 
 
 class PagedArgs(ctypes.Structure):
@@ -85,11 +89,12 @@ def new_pages(pages: int, kv_heads: int, head_dim: int, device) -> Pages:
 
 
 def _pool(p: Pages, what):
-    """(pages, kv_heads, head_dim, device index) of a pool whose tensors belong together."""
-    known = getattr(p, "_known", None)
-    if known is not None:
-        return known
+    """(pages, kv_heads, head_dim, device index, the four addresses) of a pool whose tensors belong together."""
     k, ks, v, vs = p
+    at = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
+    known = getattr(p, "_known", None)
+    if known is not None and known[4] == at:
+        return known
     if k.dim() == 4:
         pages, KV, page, hd = k.shape
         dev = k.get_device()
@@ -97,7 +102,7 @@ def _pool(p: Pages, what):
                 and k.dtype is torch.int8 and v.dtype is torch.int8 and ks.dtype is torch.float32 and vs.dtype is torch.float32
                 and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
                 and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
-            known = (pages, KV, hd, dev)
+            known = (pages, KV, hd, dev, at)
             if isinstance(p, Pages):
                 p._known = known
             return known
@@ -106,7 +111,7 @@ def _pool(p: Pages, what):
 
 
 def _args(p: Pages, pool, table, start, max_new, first, count, rows, dtype, what) -> bytes:
-    pages, KV, hd, dev = pool
+    pages, KV, hd, dev, at = pool
     if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError(f"{what}: rows are float16 or bfloat16, not {dtype}")
     if table.dim() != 2 or start.dim() != 1 or start.shape[0] != table.shape[0]:
@@ -125,7 +130,7 @@ def _args(p: Pages, pool, table, start, max_new, first, count, rows, dtype, what
     status = _status_ptr.get(dev)
     if status is None:
         status = _status_ptr[dev] = _lib.status_word(p.k.device).data_ptr()
-    return _pack(p.k.data_ptr(), p.ks.data_ptr(), p.v.data_ptr(), p.vs.data_ptr(), pages, KV, hd, table.data_ptr(), W, B, start.data_ptr(),
+    return _pack(*at, pages, KV, hd, table.data_ptr(), W, B, start.data_ptr(),
                  0 if first is None else first.data_ptr(), 0 if count is None else count.data_ptr(), max_new, rows, dtype is torch.bfloat16, status)
 
 
@@ -156,7 +161,7 @@ def append(pages: Pages, qkv, table, start, max_new: int, cos_sin, H: int, *, fi
     ``cos_sin``: :func:`kernels.rope_table`; ``rope_type`` 0 turns neighbouring dimensions, 1 the halves of a head; ``qw``, ``kw``: weights of an RMS norm of
     each head ahead of the rotation, or None.  Rows of no sequence are not written (without ``q_out`` they hold anything)."""
     pool = _pool(pages, "paged append")
-    _, KV, hd, dev = pool
+    _, KV, hd, dev, _ = pool
     if H < 1 or H % KV:
         raise ValueError(f"paged append: {H} query heads for {KV} key heads")
     rows, dtype = qkv.shape[0], qkv.dtype
@@ -182,7 +187,7 @@ def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, w
     ``start``): each sees the tokens up to its own place, the last ``window`` of them where that is not 0.  Rows of no sequence are not
     written (without ``out`` they hold anything).  ``scratch``: float32, :func:`attn_scratch` numbers, one call's at a time; without it the call allocates its own."""
     pool = _pool(pages, "paged attention")
-    _, KV, hd, dev = pool
+    _, KV, hd, dev, _ = pool
     if H < 1 or H % KV:
         raise ValueError(f"paged attention: {H} query heads for {KV} key heads")
     if not scale > 0 or window < 0:
@@ -194,6 +199,7 @@ def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, w
     B, W = table.shape
     if not (B and rows and max_new):
         return out
+    window = min(window, W * PAGE)                            # as many as there can be, and few enough for the interface's 32 bits
     L = _protos()
     need = attn_scratch(B, W, KV, hd, max_new, H, window)
     if need:
@@ -209,6 +215,7 @@ def attn(pages: Pages, q, table, start, max_new: int, H: int, scale: float, *, w
 
 def attn_scratch(B: int, width: int, kv_heads: int, head_dim: int, max_new: int, H: int, window: int = 0) -> int:
     """float32 numbers that :func:`attn` needs on the current device for ``B`` sequences with tables of ``width`` pages."""
+    window = min(window, width * PAGE)
     key = (B, width, kv_heads, head_dim, max_new, H, window, torch._C._cuda_getDevice())
     need = _scratch.get(key)
     if need is None:
@@ -227,7 +234,7 @@ def read(pages: Pages, table, start, max_new: int, dtype, rows: int, *, first=No
     """The tokens ``start[b]`` ... ``start[b] + count[b] - 1`` of the sequences as 16-bit rows: (k, v), each [rows, kv_heads, hd].  ``k_out``, ``v_out``:
     [rows, kv_heads * hd] tensors to write to."""
     pool = _pool(pages, "paged read")
-    _, KV, hd, dev = pool
+    _, KV, hd, dev, _ = pool
     if rows < 0:
         raise ValueError(f"paged read: {rows} rows")
     if dtype is not torch.float16 and dtype is not torch.bfloat16:

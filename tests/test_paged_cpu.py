@@ -1,6 +1,8 @@
 """Refusals of the paged 8-bit cache's launchers, and the arithmetic its pages rest on.  Every refusal comes before anything is launched."""
+import copy
 import ctypes
 import os
+import pickle
 
 import numpy as np
 import pytest
@@ -73,6 +75,36 @@ def test_refusals_of_rows_and_options():
             P.new_pages(4, 2, bad, "cpu")
     with pytest.raises(ValueError, match="at least one page"):
         P.new_pages(0, 2, 64, "cpu")
+
+
+def test_a_pool_that_was_good_is_checked_again_when_it_is_another():
+    p = pool()
+    with pytest.raises(ValueError, match="current device"):        # all is well but for the device
+        call("attn", p)
+    p.k.data = p.k.data[:, :1].contiguous()
+    with pytest.raises(ValueError, match="belong together"):
+        call("attn", p)
+    p = pool()
+    P._pool(p, "")
+    for q in (copy.copy(p), copy.deepcopy(p), pickle.loads(pickle.dumps(p))):
+        assert isinstance(q, P.Pages) and not hasattr(q, "_known")
+
+
+@pytest.mark.parametrize("window,least", [(2 ** 32 + 5, 3 * PAGE), (2 ** 31, 3 * PAGE), (3 * PAGE - 1, 3 * PAGE - 1), (0, 0)])
+def test_a_window_past_32_bits_is_not_a_short_one(window, least, monkeypatch):
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: seen.append((name, a)) or 0
+
+    monkeypatch.setattr(P, "_protos", Lib)
+    monkeypatch.setattr(P, "_scratch", {})
+    monkeypatch.setattr(P, "_args", lambda *a: b"")
+    monkeypatch.setattr(P, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    call("attn", window=window)
+    assert [(n, a[2] if n == "gb_paged_attn_ws" else a[5]) for n, a in seen] == [("gb_paged_attn_ws", least), ("gb_paged_attn", least)]
 
 
 @pytest.mark.skipif(not _lib.available(), reason="the kernel library is not built")
