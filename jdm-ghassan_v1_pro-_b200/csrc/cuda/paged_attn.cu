@@ -21,10 +21,10 @@ int pg_sms() {
 
 using namespace gb;
 
-// Sequences of a launch: work is dealt by places counted in 32 bits, a sequence's being at most its pages or, for every 256 query rows, its key tiles and two more.
+// Sequences of a launch: work is dealt by places counted in 32 bits, a sequence's being at most its pages or, for every 256 query rows, its pages and four more.
 static int gb_paged_most_seqs(const gb_paged* a, int H) {
   const long long items = ((long long)a->max_new * (H / a->KV) + 255) / 256;
-  const double places = (double)a->KV * items * (a->W + 2);
+  const double places = (double)a->KV * items * (a->W + 4);
   return (int)std::min<double>(PG_MOST_SEQS, 2e9 / places);
 }
 // The sequences from b0 on, as many as fit.

@@ -32,7 +32,9 @@ struct Tl {
   static constexpr int Q = 128 * 128 * PANELS, K = PG * 128 * PANELS, V = HD * 128, STAGE = K + V, STAGES = HD == 128 ? 4 : 6;
   // registers a thread: soft-max, expanding, issuing; launched with 128, so 2 x 128 x S + 128 x (E + I) is at most 65536
   static constexpr int REGS_S = 184, REGS_E = 88, REGS_I = 56;
-  static constexpr int O0 = 64 * BUFS * WGS, AHEAD = 2;       // first column of the results; places of an item ahead of its pages' (TlWalk)
+  static_assert(REGS_S >= 128 && REGS_E <= 128 && REGS_I <= 128 && 2 * 128 * REGS_S + 128 * (REGS_E + REGS_I) <= 65536 && THREADS == 512,
+                "soft-max warps take registers, the others give them, and no more than the block has");
+  static constexpr int O0 = 64 * BUFS * WGS, AHEAD = 4;       // first column of the results; places of an item ahead of its pages' (TlWalk)
   static constexpr int REC = ROWS * (HD + 2);                 // floats of a record: [HD / 4][ROWS] four results, then [ROWS] pairs (maximum, sum)
 };
 
@@ -70,7 +72,8 @@ __device__ __forceinline__ TlItem tl_item(const PgAttn& p, const PgSeq& s, int G
 }
 
 // A block's walk over its run: places f ... end, one piece of an item after the other.  An item has a place for each page and, ahead of them, AHEAD for its start and end: loading queries,
-// filling and emptying the pipelines take as long as two pages.
+// filling and emptying the pipelines, and the last pages' masks.  Four of them: 7 ragged prompts (12/4 heads of 64) 184 us, 2 of them 196, 3 of them 190, 6 of them 184; a prompt of 2048 tokens
+// 32.8, 37.4, 33.3, 34.2.
 template <int ROWS, int AHEAD>
 struct TlWalk {
   int f, end, b, g, qt, k;                                    // k: places of the item that come before place f
