@@ -70,8 +70,10 @@ __global__ void __launch_bounds__(256) moe_route_kernel(const gb_moe_args a) {
     const float p0 = e0 * inv, p1 = e1 * inv;
     if (lane < ne) a.probs[(size_t)t * ne + lane] = p0;
     if (lane + 32 < ne) a.probs[(size_t)t * ne + lane + 32] = p1;
-    float s0 = lane < ne ? p0 + (a.bias ? a.bias[lane] : 0.f) : -INFINITY;
-    float s1 = lane + 32 < ne ? p1 + (a.bias ? a.bias[lane + 32] : 0.f) : -INFINITY;
+    // A score that is NaN counts as the least number: comparisons with NaN are false, every lane would take itself for the winner and nobody be left for the next
+    // pick.  A token's experts have to be there and to differ, whatever its row holds: the sorted copy has a place for each.
+    float s0 = lane < ne ? fmaxf(p0 + (a.bias ? a.bias[lane] : 0.f), -3.4028235e38f) : -INFINITY;
+    float s1 = lane + 32 < ne ? fmaxf(p1 + (a.bias ? a.bias[lane + 32] : 0.f), -3.4028235e38f) : -INFINITY;
     float psel[MAX_K];
     int esel[MAX_K];
     float psum = 0.f;
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(RT_THREADS) moe_route_tc_kernel(const __grid_c
         for (int e = 0; e < 8; ++e) {
           pr[e] *= inv;
           if (e < ne) a.probs[(size_t)t * ne + e] = pr[e];
-          sc[e] = e < ne ? pr[e] + (a.bias ? a.bias[e] : 0.f) : -INFINITY;
+          sc[e] = e < ne ? fmaxf(pr[e] + (a.bias ? a.bias[e] : 0.f), -3.4028235e38f) : -INFINITY;   // NaN: the least number (above)
         }
         int esel[MAX_K];
         float psel[MAX_K];

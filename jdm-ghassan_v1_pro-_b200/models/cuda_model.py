@@ -419,7 +419,7 @@ class CudaModel:
         cfg = self.cfg
         qd, kvd, H, KV, hd = cfg.q_dim, cfg.kv_dim, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         sink = getattr(self, "kv_sink", None)
-        if sink is not None and sink.paged:      # rows past the prompt are not written: what is there is finite (zeros, or an earlier prompt's rows)
+        if sink is not None and sink.paged:      # rows past the prompt are not written: they hold zeros or an earlier prompt's rows, and no other row sees them
             sink.paged_prompt(sink.layers[l], b.qkv, b.qk[:, :qd], b.att)
             return
         K.qk_norm_rope_fwd(b.qkv, b.qk, qw, kw, self.cos_sin, self.pos, H, KV, hd, cfg.rms_eps, cfg.rope_type)

@@ -220,6 +220,31 @@ def test_moe_route_group_matches_reference(n, ne, Kk, shared, jit, d):
         assert float(xp[so[e] + tot[e]:so[e + 1]].abs().max() if so[e + 1] > so[e] + tot[e] else 0) == 0.0
 
 
+@pytest.mark.parametrize("n,ne,Kk,d", [(100, 8, 2, 256), (40, 5, 3, 264), (300, 64, 8, 512), (300, 8, 2, 128)])
+def test_router_rows_that_are_not_numbers(n, ne, Kk, d):
+    """Such a row still goes to experts that there are, with weights that are not numbers; the other rows' choices are what they were."""
+    k = K()
+    x16, rw = _moe_setup(n, d, ne, Kk, True)
+    got = []
+    for spoil in (False, True):
+        x = x16.clone()
+        if spoil:
+            x[3, 5] = float("nan")
+            x[17] = float("nan")
+            x[n - 1, 0] = float("inf")
+        ws = k.MoeWorkspace(n, d, ne, Kk, True, torch.float16, "cuda")
+        xp = torch.zeros(ws.cap, d, dtype=torch.float16, device="cuda")
+        k.moe_route_group(ws, x, rw, None, xp, None)
+        torch.cuda.synchronize()
+        assert int(ws.idx.min()) >= 0 and int(ws.idx.max()) < ne
+        assert int(ws.slot_pos.min()) >= 0 and int(ws.slot_pos.max()) < ws.cap
+        got.append((ws.idx.clone(), ws.w.clone()))
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[[3, 17, n - 1]] = True
+    assert torch.isnan(got[1][1][bad]).all()
+    assert torch.equal(got[0][0][~bad], got[1][0][~bad]) and torch.equal(got[0][1][~bad], got[1][1][~bad])
+
+
 @pytest.mark.parametrize("n, ne, Kk, shared", [(1, 8, 2, True), (9, 8, 1, False), (6144, 8, 2, True), (6145, 8, 2, True), (8191, 2, 1, True),
                                               (8192, 8, 4, True), (33000, 8, 2, False), (2000, 64, 6, True), (840, 64, 2, False)])
 def test_moe_grouping_beside_its_scan(n, ne, Kk, shared):
