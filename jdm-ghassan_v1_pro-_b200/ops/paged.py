@@ -30,19 +30,13 @@ PAGE = 64
 HEAD_DIMS = (32, 64, 128)
 
 
-class _PoolTensors(NamedTuple):
+class Pages(NamedTuple):
+    """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads],
+    powers of two."""
     k: torch.Tensor
     ks: torch.Tensor
     v: torch.Tensor
     vs: torch.Tensor
-
-
-class Pages(_PoolTensors):
-    """One layer's pool: codes ``k`` int8 [pages, kv_heads, 64, head_dim] and ``v`` int8 [pages, kv_heads, head_dim, 64], scales ``ks`` and ``vs`` fp32 [pages, kv_heads],
-    powers of two.  A call checks that they belong together, unless they are where they were when an earlier one did."""
-
-    def __reduce__(self):                                     # copies and what is loaded from a file are checked anew
-        return Pages, tuple(self)
 
 
 class PagedArgs(ctypes.Structure):
@@ -89,12 +83,9 @@ def new_pages(pages: int, kv_heads: int, head_dim: int, device) -> Pages:
 
 
 def _pool(p: Pages, what):
-    """(pages, kv_heads, head_dim, device index, the four addresses) of a pool whose tensors belong together."""
+    """(pages, kv_heads, head_dim, device index, the four addresses) of a pool whose tensors belong together: every call looks, since a tensor can be resized or
+    replaced in place, and the kernels write to wherever its sizes say."""
     k, ks, v, vs = p
-    at = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
-    known = getattr(p, "_known", None)
-    if known is not None and known[4] == at:
-        return known
     if k.dim() == 4:
         pages, KV, page, hd = k.shape
         dev = k.get_device()
@@ -102,10 +93,7 @@ def _pool(p: Pages, what):
                 and k.dtype is torch.int8 and v.dtype is torch.int8 and ks.dtype is torch.float32 and vs.dtype is torch.float32
                 and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
                 and v.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
-            known = (pages, KV, hd, dev, at)
-            if isinstance(p, Pages):
-                p._known = known
-            return known
+            return pages, KV, hd, dev, (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
     raise ValueError(f"{what}: the pool's tensors do not belong together: contiguous int8 codes [pages, kv_heads, 64, head_dim] and [pages, kv_heads, head_dim, 64], float32 "
                      f"scales [pages, kv_heads], on one device; got " + ", ".join(f"{tuple(t.shape)} {t.dtype} on {t.device}" for t in p))
 

@@ -90,6 +90,30 @@ def test_a_pool_that_was_good_is_checked_again_when_it_is_another():
         assert isinstance(q, P.Pages) and not hasattr(q, "_known")
 
 
+def test_a_pool_that_changed_in_place_is_another():
+    """Tensors that are where they were, with another number of pages, type or order: nothing of an earlier call's check is kept."""
+    def halved(t):
+        t.resize_(2, *t.shape[1:])
+
+    def turned(t):
+        t.transpose_(0, 1)
+
+    def retyped(t):
+        t.data = t.data.view(torch.uint8 if t.dtype == torch.int8 else torch.int32)
+
+    for change in (halved, turned, retyped):
+        for i in range(4):
+            p = pool()
+            with pytest.raises(ValueError, match="current device"):    # all is well but for the device
+                call("attn", p)
+            at = p[i].data_ptr()
+            change(p[i])
+            assert p[i].data_ptr() == at
+            for name in ("append", "attn", "read"):
+                with pytest.raises(ValueError, match="belong together"):
+                    call(name, p)
+
+
 @pytest.mark.parametrize("window,least", [(2 ** 32 + 5, 3 * PAGE), (2 ** 31, 3 * PAGE), (3 * PAGE - 1, 3 * PAGE - 1), (0, 0)])
 def test_a_window_past_32_bits_is_not_a_short_one(window, least, monkeypatch):
     seen = []
