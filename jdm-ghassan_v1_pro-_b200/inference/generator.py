@@ -157,7 +157,7 @@ class Generator:
         reasons = ["length"] * B
         streams = [self.tok.stream() if self.tok is not None else None for _ in range(B)]
         text_so_far = [""] * B
-        for _ in range(max_new):
+        for step in range(max_new):
             logits = eng.logits.cpu().numpy()
             nxt = []
             for b in range(B):
@@ -177,7 +177,7 @@ class Generator:
                         on_text(b, piece)
                     if any(s and s in text_so_far[b] for s in stop_strings):
                         done[b], reasons[b] = True, "stop_string"
-            if all(done):
+            if all(done) or step + 1 == max_new:              # nobody asks what follows the last token, and its keys may have no place
                 break
             eng.cur_tok.copy_(torch.tensor(nxt, dtype=torch.int32))
             eng._forward_token()
@@ -263,8 +263,8 @@ class Generator:
         t1 = time.perf_counter()
         toks, _ = self._run_host(sp, [list(map(int, p)) for p in prompt], new_tokens, set(), (), None)
         t2 = time.perf_counter()
-        n = sum(len(t) for t in toks)
+        steps = max(1, new_tokens - 1)                        # the first token's pass is the prompt's
         return {"batch": eng.B, "prompt_len": prompt_len, "new_tokens": new_tokens,
-                "decode_ms_per_token": (t2 - t1) * 1e3 / max(1, new_tokens), "decode_tokens_per_s": n / max(1e-9, t2 - t1),
+                "decode_ms_per_token": (t2 - t1) * 1e3 / steps, "decode_tokens_per_s": steps * eng.B / max(1e-9, t2 - t1),
                 "stored_weight_bytes": eng.weight_bytes, "prefill_ms": (t1 - t0) * 1e3,
                 "distinct_tokens": int(len({t for row in toks for t in row})), "device": "cpu"}
