@@ -102,6 +102,8 @@ class TokenLoop:
         """Run ``n`` decode steps (forward of ``cur_tok`` + sampling of the next token) without host reads."""
         if not sp.device_ok():
             raise ValueError("these sampling settings need the host sampler: use Generator.generate")
+        if n <= 0:
+            return
         key = (sp.temperature, sp.top_k, sp.top_p, sp.min_p, sp.repetition_penalty, sp.repetition_window,
                sp.frequency_penalty, sp.presence_penalty, sp.greedy, self.n_stop)
         self._draw_uniforms(n)

@@ -62,3 +62,22 @@ def test_a_sequence_that_stops_early_does_not_end_the_others():
     eng = Counting(12, batch=2)
     res = Generator(eng).generate([[0, 1], [5, 6]], max_new_tokens=64, sampling=SamplingParams(no_repeat_ngram=3, **HOST), stop_tokens=[4])
     assert res.tokens == [[2, 3], list(range(7, 18))] and res.stopped == ["eos", "length"] and eng.passes == 12
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_no_steps_are_no_steps(graph):
+    """With settings that no captured step has yet, too: the step that precedes a capture is one of those asked for."""
+    class Loop(TokenLoop):
+        graph, _graph_key, n_stop, ran = None, None, 0, 0
+
+        def _draw_uniforms(self, n):
+            pass
+
+        def _step_eager(self, sp):
+            self.ran += 1
+
+    loop = Loop()
+    loop.decode_steps(0, SamplingParams(greedy=True), use_graph=graph)
+    assert loop.ran == 0 and loop.graph is None
+    with pytest.raises(ValueError, match="host sampler"):
+        loop.decode_steps(0, SamplingParams(top_k=0), use_graph=graph)
