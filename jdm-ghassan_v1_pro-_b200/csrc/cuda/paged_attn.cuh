@@ -26,6 +26,9 @@ __device__ __forceinline__ float pg_ex2(float x) {
   return r;
 }
 
+// 2^x of a whole number up to 127; 0 where that is no normal number
+__device__ __forceinline__ float pg_pow2(float x) { return x < -126.f ? 0.f : __uint_as_float((uint32_t)((int)x + 127) << 23); }
+
 // 4 codes (a little-endian word) as two pairs of float16: the bytes, raised by 128, under the exponent of 1024, which is 1024 + 128 + code
 __device__ __forceinline__ void pg_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
   const uint32_t u = w ^ 0x80808080u;

@@ -5,8 +5,8 @@
 // scores, maxima, exponentials and products (2600 cycles, of which two warpgroups' exponentials are 1024).
 //
 // One block an SM: two warpgroups of soft-max threads, a row each; four warps expand the pages from codes in global memory to float16 integers in the swizzled layout of the MMAs
-// (integers up to 127 are exact, the scales go into the soft-max: a key scale into the score's factor, a value scale into the weight's exponent, as in paged_attn_token.cu); a warp for
-// each warpgroup issues (one for both was busy issuing and asking barriers all the time).  Scores and weights share tensor memory: weights go over scores that have been read,
+// (integers up to 127 are exact, the scales go into the soft-max: a key scale into the score's factor, a value scale into the weight's exponent, as in paged_attn_token.cu, but that a
+// row's largest weight is held as 2^6 to 2^15, so that one is off by 2^-31 of the largest where that is more than half a step of 2^-11 of itself); a warp for each warpgroup issues (one for both was busy issuing and asking barriers all the time).  Scores and weights share tensor memory: weights go over scores that have been read,
 // and are the A operand of the second product from there.
 //
 // The work is dealt in pages: all (sequence, key head, item, page) in a row are cut into equal runs, one a block.  Items that a cut goes through leave records
@@ -19,6 +19,7 @@
 namespace gb {
 
 constexpr float TL_OFF = 7.f, TL_LAZY = 8.f;   // weights are held as 2^7 of themselves and may grow 2^8 before the sums are rescaled
+constexpr float TL_NONE = -1000.f;             // less than any exponent of a value scale
 
 template <int HD>
 struct Tl {
@@ -248,8 +249,9 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&q_full[wg]);
-          float m2 = -1e30f, l = 0.f;
-          int E = -1000;
+          // soft-max of 2^s: m2, the running maximum (or up to TL_LAZY less), to which l is the sum; m2 + rel, that of s + e, with e a value scale's exponent, to which the
+          // weights and the results are (d, which is rel rounded up): what a row does not see, or gives no weight, does not move either
+          float m2 = -1e30f, rel = TL_NONE, l = 0.f;
           for (int t = k0; t < k1; ++t, ++it, ++kv_it) {
             const uint32_t buf = it % L::BUFS, phase = (it / L::BUFS) & 1u;
             const uint32_t tS = tmem + wg * (64 * L::BUFS) + buf * 64 + row;
@@ -299,15 +301,18 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
             float f = qs * fabsf(sc.x);
             f = f == 0.f ? 1e-37f : f;
             top *= f;
-            const int ev = (int)(__float_as_uint(sc.y) >> 23) - 127, En = max(E, ev);
-            if (__any_sync(0xffffffffu, top > m2 + TL_LAZY || En != E)) {
-              const float mn = fmaxf(m2, top), corr = pg_ex2(m2 - mn);
-              l *= corr;
+            const float ev = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
+            float d = ceilf(rel);
+            if (__any_sync(0xffffffffu, fmaxf(top - m2, top - m2 + (ev - d)) > TL_LAZY)) {
+              const float mn = fmaxf(m2, top), down = m2 - mn, was = d;
+              l *= pg_ex2(down);
               m2 = mn;
+              rel = fmaxf(rel + down, ev + (top - mn));                   // where all of the page is hidden top is -inf
+              d = ceilf(rel);
               if (t > k0) {                                    // what the pages before added up to is rescaled, once it is there
                 if (!tl_wait(&o_full[wg * L::BUFS + (it - 1u) % L::BUFS], ((it - 1u) / L::BUFS) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const float c2 = corr * exp2f((float)(E - En));
+                const float c2 = pg_ex2(down + (was - d));
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
                   uint32_t rg[16];
@@ -318,9 +323,8 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
                   tmem_st_32x16(tO + c * 16, rg);
                 }
               }
-              E = En;
             }
-            const float de = fmaxf((float)(ev - En), -60.f);
+            const float de = fmaxf(ev - d, -60.f);                        // no less, so that the row sum gets all weights: 2^-60 of the page's values is nothing
             const float2 ff = make_float2(f, f), bias = make_float2(TL_OFF + de - m2, TL_OFF + de - m2);
             float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
               }
               tmem_st_32x16(tS + c * 16, pk);
             }
-            l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), exp2f(-de), l);
+            l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), pg_ex2(-de), l);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -349,7 +353,7 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
           const bool whole = k0 == 0 && k1 == item.n;
           const int f0 = w.f - w.k + L::AHEAD, slot = 2 * blockIdx.x + (f0 > start.f ? 1 : 0);
           float* rec = records + (size_t)slot * L::REC;
-          const float fac = l == 0.f ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23) / l;
+          const float inv = l == 0.f ? 0.f : 1.f / l, unit = pg_pow2(ceilf(rel));       // 2^d / l, in two steps: together they may be less than fp32 has
           T* dst = reinterpret_cast<T*>(p.out) + (long long)(w.s.first + i) * p.ld_o + (long long)(w.g * G + rr - i * G) * HD;
 #pragma unroll
           for (int c = 0; c < HD / 32; ++c) {
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
             tmem_ld_wait();
             float v[32];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(rg[k]) * fac;
+            for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(rg[k]) * inv * unit;
             if (whole) {
               if (row_ok) {
 #pragma unroll

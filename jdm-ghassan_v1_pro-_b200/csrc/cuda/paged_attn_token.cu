@@ -10,8 +10,9 @@
 // A page is two products on the legacy tensor path, with the codes as float16 integers (exact): keys x queries and values x weights, so that
 // queries (8 columns) rather than keys are padded; 16 rows of queries would pad 3 of them to 16.  The order of the contracted dimensions is free as long as both operands have the
 // same, so a lane takes 16 consecutive bytes of a key, or of a value's tokens, and these are its MMA fragments.  The page's key scale joins the score's factor and its value
-// scale the exponent of the weights: w = 2^(s - m + 15 + e - E), with m the running maximum, e the value scale's exponent and E the largest so far.  Rounded to float16 a
-// weight is off by 2^-11 of itself, or by 2^-39 of the largest page's, whichever is more; the row sum has the unrounded weights.  Queries are scaled by a power of two so that a
+// scale the exponent of the weights: w = 2^(s - m + 15 + e - d), with m the row's running maximum, e the value scale's exponent and m + d the running maximum of s + e, rounded up: what a
+// row does not see, or gives no weight, does not move its d, however large its values are.  Rounded to float16 a weight is off by half a step of 2^-11 of itself, or by 2^-39 of the
+// largest 2^(s + e - d) that the row sees, whichever is more; the row sum has the unrounded weights.  Queries are scaled by a power of two so that a
 // row's largest is between 2^14 and 2^15: float16 then holds them as exactly as bfloat16 does.
 #include <algorithm>
 
@@ -24,7 +25,8 @@ constexpr int TK_WARPS = 8, TK_THREADS = 32 * TK_WARPS;
 // token behind 4, 8, 16, 24, 32 and 64 pages: one sequence 4.9, 5.4, 6.8, 8.3, 9.9, 16.1 against 7.0, 6.8, 8.2, 8.4, 8.6, 9.0; 32 sequences as long as each other gain more
 // (10.4 against 12.2 at 32 pages), but lengths are on the device and blocks of a ragged batch wait for the longest.
 constexpr int TK_ITEM_PAGES = 16;
-constexpr float TK_OFF = 15.f;               // weights are held as 2^15 of themselves, the most float16 takes
+constexpr float TK_OFF = 15.f;               // the largest weight is held as 2^15 or (d is rounded up) a little less, the most float16 takes
+constexpr float TK_NONE = -1000.f;           // less than any exponent of a value scale
 
 __device__ __forceinline__ void tk_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -151,8 +153,8 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   };
 
   uint32_t qf[NQ][KK][2];
-  float qs[NQ][2], m[NQ][2], l[NQ][2], o[NQ][KK][4];
-  int E = -1000, item = -1, pos0 = 0, n_new = 0, f_begin = 0, f_end = 0;
+  float qs[NQ][2], m[NQ][2], l[NQ][2], rel[NQ][2], o[NQ][KK][4];   // rel: the largest s + e so far, less m; d is rel rounded up
+  int item = -1, pos0 = 0, n_new = 0, f_begin = 0, f_end = 0;
   PgSeq sq{0, 0, 0};
 
   // A lane has HD / 4 numbers of its rows, where it has them of a key.  Those of the warp's first item are asked for ahead of all else.
@@ -200,13 +202,13 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         qs[q][c] = __shfl_sync(0xffffffffu, f, (2 * tq + c) * 4);
         m[q][c] = -1e30f;
         l[q][c] = 0.f;
+        rel[q][c] = TK_NONE;
       }
 #pragma unroll
       for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[q][k][c] = 0.f;
     }
-    E = -1000;
   };
 
   // the piece at hand is over: to the output where it is the whole item, else into a record
@@ -215,7 +217,6 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
     const int rows = sq.n * G;
     const bool whole = f_begin >= w_lo && f_end <= w_hi, first = f_begin <= w_lo;
     float* rec = first ? heads + warp * rec_n : reinterpret_cast<float*>(ring);
-    const float unit = E < -500 ? 0.f : __uint_as_float((uint32_t)(E + 127) << 23);
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
 #pragma unroll
@@ -224,22 +225,23 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         s += __shfl_xor_sync(0xffffffffu, s, 4);
         s += __shfl_xor_sync(0xffffffffu, s, 8);
         s += __shfl_xor_sync(0xffffffffu, s, 16);
-        const float f = s == 0.f ? 0.f : __fdividef(unit, s);
+        // 2^d / s, in two steps: together they may be less than fp32 has
+        const float f = s == 0.f ? 0.f : __fdividef(1.f, s), unit = pg_pow2(ceilf(rel[q][c]));
         const int r = 8 * q + 2 * tq + c;
         if (r >= rows) continue;
         if (whole) {
           T* dst = tk_out<T, HD>(p, sq.first, g_base + item % KVs, rows_of[r]) + gq;
 #pragma unroll
           for (int k = 0; k < KK; ++k) {
-            dst[16 * k] = Cvt<T>::from_f(o[q][k][c] * f);
-            dst[16 * k + 8] = Cvt<T>::from_f(o[q][k][2 + c] * f);
+            dst[16 * k] = Cvt<T>::from_f(o[q][k][c] * f * unit);
+            dst[16 * k + 8] = Cvt<T>::from_f(o[q][k][2 + c] * f * unit);
           }
         } else {
           float* dst = rec + r * HD + gq;
 #pragma unroll
           for (int k = 0; k < KK; ++k) {
-            dst[16 * k] = o[q][k][c] * f;
-            dst[16 * k + 8] = o[q][k][2 + c] * f;
+            dst[16 * k] = o[q][k][c] * f * unit;
+            dst[16 * k + 8] = o[q][k][2 + c] * f * unit;
           }
           if (gq == 0) *reinterpret_cast<float2*>(rec + R * HD + 2 * r) = make_float2(m[q][c], s);
         }
@@ -365,15 +367,13 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
             f[q][c] = 1.f;
           }
       }
-      const int ev = (int)(__float_as_uint(vs) >> 23) - 127, En = max(E, ev);
-      const float shrink = E == En ? 1.f : exp2f((float)(E - En));
-      const float de = fmaxf((float)(ev - En), -60.f), up = exp2f(-de);
-      bool same = E == En;
+      const float ev = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+      bool same = true;
       uint32_t pb[NQ][4][2];
-      float corr[NQ][2];
+      float corr[NQ][2], scale_o[NQ][2];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        float mn[2], sum[2];
+        float mn[2], de[2], sum[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float x = fmaxf(fmaxf(fmaxf(s[q][0][c], s[q][0][2 + c]), fmaxf(s[q][1][c], s[q][1][2 + c])),
@@ -381,9 +381,15 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          mn[c] = fmaxf(m[q][c], x * f[q][c]);
-          corr[q][c] = pg_ex2(m[q][c] - mn[c]);
-          same = same && mn[c] == m[q][c];
+          x *= f[q][c];
+          mn[c] = fmaxf(m[q][c], x);
+          const float was = ceilf(rel[q][c]), down = m[q][c] - mn[c];
+          rel[q][c] = fmaxf(rel[q][c] + down, ev + (x - mn[c]));       // where all of the page is hidden x is -inf
+          const float d = ceilf(rel[q][c]);
+          de[c] = fmaxf(ev - d, -60.f);                                // no less, so that the row sum gets all weights: 2^-60 of the page's values is nothing
+          corr[q][c] = pg_ex2(down);
+          scale_o[q][c] = pg_ex2(down + (was - d));
+          same = same && down == 0.f && was == d;
           m[q][c] = mn[c];
           sum[c] = 0.f;
         }
@@ -391,27 +397,23 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float w0 = pg_ex2(fmaf(s[q][j][2 * e], f[q][0], TK_OFF + de - mn[0]));
-            const float w1 = pg_ex2(fmaf(s[q][j][2 * e + 1], f[q][1], TK_OFF + de - mn[1]));
+            const float w0 = pg_ex2(fmaf(s[q][j][2 * e], f[q][0], TK_OFF + de[0] - mn[0]));
+            const float w1 = pg_ex2(fmaf(s[q][j][2 * e + 1], f[q][1], TK_OFF + de[1] - mn[1]));
             sum[0] += w0;
             sum[1] += w1;
             pb[q][j][e] = tk_transpose(Cvt<__half>::pack2(w0, w1));
           }
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          l[q][c] = fmaf(l[q][c], corr[q][c], sum[c] * up);
-          corr[q][c] *= shrink;
-        }
+        for (int c = 0; c < 2; ++c) l[q][c] = fmaf(l[q][c], corr[q][c], sum[c] * pg_ex2(-de[c]));
       }
-      E = En;
       if (__any_sync(0xffffffffu, !same)) {
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
           for (int k = 0; k < KK; ++k)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[q][k][c] *= corr[q][c & 1];
+            for (int c = 0; c < 4; ++c) o[q][k][c] *= scale_o[q][c & 1];
       }
       // ---- values: o[q][k]: dimensions 16k + g, 16k + g + 8, queries 2t, 2t + 1
       wait_or_report(&bar[slot_out], parity, a.status, ST_TIMEOUT_FULL, abort_flag);

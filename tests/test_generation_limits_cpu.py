@@ -81,3 +81,12 @@ def test_no_steps_are_no_steps(graph):
     assert loop.ran == 0 and loop.graph is None
     with pytest.raises(ValueError, match="host sampler"):
         loop.decode_steps(0, SamplingParams(top_k=0), use_graph=graph)
+
+
+def test_scoring_asks_whether_the_cache_held_what_it_was_given():
+    eng = Counting(50)
+    nll, n = Generator(eng).score_tokens([1, 2, 3, 4])
+    assert n == 3 and nll < 1e-3 and len(eng.told) == 1
+    eng.paged = False                                         # the other engines have no such question
+    Generator(eng).score_tokens([1, 2, 3, 4])
+    assert len(eng.told) == 1
