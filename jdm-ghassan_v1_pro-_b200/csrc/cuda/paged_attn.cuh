@@ -26,6 +26,10 @@ __device__ __forceinline__ float pg_ex2(float x) {
   return r;
 }
 
+constexpr float PG_START = -1e30f;           // a running maximum before its first score
+// A maximum that a weight's exponent (offset + value scale - maximum, a few hundred) is not added to in one step: an fp32 number past 2^8 has steps of 2^-15 and more.
+__device__ __forceinline__ bool pg_far(float m) { return fabsf(m) > 256.f && m != PG_START; }
+
 // 2^x of a whole number up to 127; 0 where that is no normal number
 __device__ __forceinline__ float pg_pow2(float x) { return x < -126.f ? 0.f : __uint_as_float((uint32_t)((int)x + 127) << 23); }
 

@@ -251,7 +251,8 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
           if (lane == 0) mbar_arrive(&q_full[wg]);
           // soft-max of 2^s: m2, the running maximum (or up to TL_LAZY less), to which l is the sum; m2 + rel, that of s + e, with e a value scale's exponent, to which the
           // weights and the results are (d, which is rel rounded up): what a row does not see, or gives no weight, does not move either
-          float m2 = -1e30f, rel = TL_NONE, l = 0.f;
+          float m2 = PG_START, rel = TL_NONE, l = 0.f;
+          bool far = false;
           for (int t = k0; t < k1; ++t, ++it, ++kv_it) {
             const uint32_t buf = it % L::BUFS, phase = (it / L::BUFS) & 1u;
             const uint32_t tS = tmem + wg * (64 * L::BUFS) + buf * 64 + row;
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
             // a factor that is too small for fp32 must not make nothing of a hidden score
             float f = qs * fabsf(sc.x);
             f = f == 0.f ? 1e-37f : f;
-            top *= f;
+            top = __fmul_ru(top, f);                           // never less than the score that the weights are found from
             const float ev = (float)((int)(__float_as_uint(sc.y) >> 23) - 127);
             float d = ceilf(rel);
             if (__any_sync(0xffffffffu, fmaxf(top - m2, top - m2 + (ev - d)) > TL_LAZY)) {
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
               m2 = mn;
               rel = fmaxf(rel + down, ev + (top - mn));                   // where all of the page is hidden top is -inf
               d = ceilf(rel);
+              far = __any_sync(0xffffffffu, pg_far(m2));
               if (t > k0) {                                    // what the pages before added up to is rescaled, once it is there
                 if (!tl_wait(&o_full[wg * L::BUFS + (it - 1u) % L::BUFS], ((it - 1u) / L::BUFS) & 1u, a.status, ST_TIMEOUT_TMEM_FULL, abort_flag)) { ok = false; break; }
                 tc_fence_after();
@@ -325,7 +327,17 @@ __global__ void __launch_bounds__(Tl<HD>::THREADS, 1) paged_tile_kernel(const __
               }
             }
             const float de = fmaxf(ev - d, -60.f);                        // no less, so that the row sum gets all weights: 2^-60 of the page's values is nothing
-            const float2 ff = make_float2(f, f), bias = make_float2(TL_OFF + de - m2, TL_OFF + de - m2);
+            float2 ff = make_float2(f, f), bias = make_float2(TL_OFF + de - m2, TL_OFF + de - m2);
+            if (far) {                                           // scores less their maximum first: it would swallow the rest of the exponent
+#pragma unroll
+              for (int j = 0; j < 64; j += 2) {
+                const float2 y = tl_fma2(make_float2(x[j], x[j + 1]), ff, make_float2(-m2, -m2));
+                x[j] = y.x;
+                x[j + 1] = y.y;
+              }
+              ff = make_float2(1.f, 1.f);
+              bias = make_float2(TL_OFF + de, TL_OFF + de);
+            }
             float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {

@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
   float qs[NQ][2], m[NQ][2], l[NQ][2], rel[NQ][2], o[NQ][KK][4];   // rel: the largest s + e so far, less m; d is rel rounded up
   int item = -1, pos0 = 0, n_new = 0, f_begin = 0, f_end = 0;
   PgSeq sq{0, 0, 0};
+  bool far = false;                           // a maximum is large (pg_far)
 
   // A lane has HD / 4 numbers of its rows, where it has them of a key.  Those of the warp's first item are asked for ahead of all else.
   uint4 raw[NQ][HD / 32];
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
 #pragma unroll
       for (int c = 0; c < 2; ++c) {           // the factor where scores have it: lanes of queries 2t, 2t + 1
         qs[q][c] = __shfl_sync(0xffffffffu, f, (2 * tq + c) * 4);
-        m[q][c] = -1e30f;
+        m[q][c] = PG_START;
         l[q][c] = 0.f;
         rel[q][c] = TK_NONE;
       }
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[q][k][c] = 0.f;
     }
+    far = false;
   };
 
   // the piece at hand is over: to the output where it is the whole item, else into a record
@@ -362,18 +364,17 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
               for (int e = 0; e < 2; ++e) {
                 const int key = pg * PG + 16 * (gq >> 1) + 4 * j + (gq & 1) + 2 * e;
                 const bool see = !all_bad && key <= pos && (p.window <= 0 || key > pos - p.window);
-                s[q][j][2 * e + c] = see ? s[q][j][2 * e + c] * f[q][c] : -INFINITY;
+                s[q][j][2 * e + c] = see ? s[q][j][2 * e + c] : -INFINITY;
               }
-            f[q][c] = 1.f;
+            f[q][c] = f[q][c] == 0.f ? 1e-37f : f[q][c];       // a factor that is too small for fp32 must not make a number of a hidden score
           }
       }
       const float ev = (float)((int)(__float_as_uint(vs) >> 23) - 127);
       bool same = true;
       uint32_t pb[NQ][4][2];
-      float corr[NQ][2], scale_o[NQ][2];
+      float corr[NQ][2], scale_o[NQ][2], de[NQ][2];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        float mn[2], de[2], sum[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float x = fmaxf(fmaxf(fmaxf(s[q][0][c], s[q][0][2 + c]), fmaxf(s[q][1][c], s[q][1][2 + c])),
@@ -381,39 +382,64 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x *= f[q][c];
-          mn[c] = fmaxf(m[q][c], x);
-          const float was = ceilf(rel[q][c]), down = m[q][c] - mn[c];
-          rel[q][c] = fmaxf(rel[q][c] + down, ev + (x - mn[c]));       // where all of the page is hidden x is -inf
+          x = __fmul_ru(x, f[q][c]);                                   // never less than the score that the weights are found from
+          const float mn = fmaxf(m[q][c], x), was = ceilf(rel[q][c]), down = m[q][c] - mn;
+          rel[q][c] = fmaxf(rel[q][c] + down, ev + (x - mn));          // where all of the page is hidden x is -inf
           const float d = ceilf(rel[q][c]);
-          de[c] = fmaxf(ev - d, -60.f);                                // no less, so that the row sum gets all weights: 2^-60 of the page's values is nothing
+          de[q][c] = fmaxf(ev - d, -60.f);                             // no less, so that the row sum gets all weights: 2^-60 of the page's values is nothing
           corr[q][c] = pg_ex2(down);
           scale_o[q][c] = pg_ex2(down + (was - d));
           same = same && down == 0.f && was == d;
-          m[q][c] = mn[c];
-          sum[c] = 0.f;
+          m[q][c] = mn;
         }
+      }
+      if (__any_sync(0xffffffffu, !same)) {
+        bool some = false;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          some = some || pg_far(m[q][0]) || pg_far(m[q][1]);
+#pragma unroll
+          for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[q][k][c] *= scale_o[q][c & 1];
+        }
+        far = __any_sync(0xffffffffu, some);
+      }
+      float base[NQ][2];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) base[q][c] = TK_OFF + de[q][c] - m[q][c];
+      if (far) {                                                       // scores less their maximum first: it would swallow the rest of the exponent
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s[q][j][c] = fmaf(s[q][j][c], f[q][c], -m[q][c]);
+              s[q][j][2 + c] = fmaf(s[q][j][2 + c], f[q][c], -m[q][c]);
+            }
+            f[q][c] = 1.f;
+            base[q][c] = TK_OFF + de[q][c];
+          }
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float w0 = pg_ex2(fmaf(s[q][j][2 * e], f[q][0], TK_OFF + de[0] - mn[0]));
-            const float w1 = pg_ex2(fmaf(s[q][j][2 * e + 1], f[q][1], TK_OFF + de[1] - mn[1]));
+            const float w0 = pg_ex2(fmaf(s[q][j][2 * e], f[q][0], base[q][0]));
+            const float w1 = pg_ex2(fmaf(s[q][j][2 * e + 1], f[q][1], base[q][1]));
             sum[0] += w0;
             sum[1] += w1;
             pb[q][j][e] = tk_transpose(Cvt<__half>::pack2(w0, w1));
           }
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) l[q][c] = fmaf(l[q][c], corr[q][c], sum[c] * pg_ex2(-de[c]));
-      }
-      if (__any_sync(0xffffffffu, !same)) {
-#pragma unroll
-        for (int q = 0; q < NQ; ++q)
-#pragma unroll
-          for (int k = 0; k < KK; ++k)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[q][k][c] *= scale_o[q][c & 1];
+        for (int c = 0; c < 2; ++c) l[q][c] = fmaf(l[q][c], corr[q][c], sum[c] * pg_ex2(-de[q][c]));
       }
       // ---- values: o[q][k]: dimensions 16k + g, 16k + g + 8, queries 2t, 2t + 1
       wait_or_report(&bar[slot_out], parity, a.status, ST_TIMEOUT_FULL, abort_flag);

@@ -119,3 +119,16 @@ def test_a_missing_page_does_not_count(n, width):
     r = np.random.default_rng(n)
     k, v = (r.standard_normal((400, 2, 64)) for _ in range(2))
     check(pages_of(k, v * 2.0 ** -50), r.standard_normal((n, 4, 64)), 400 - n, 0.125, 0, "bf16", missing=(2,), status=301, width=width)
+
+
+@pytest.mark.parametrize("n", [1, 5, 70])
+@pytest.mark.parametrize("size", [20.0, 300.0, 2000.0, -20.0, -300.0, -2000.0])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_scores_that_leave_fp32_few_bits(n, size, width):
+    """Equal keys and scores of 4.6e3, 1e6 and 4.6e7 in powers of two: weights are equal, whatever their page's value scale.  The last key of every second page scores 1 % less."""
+    r = np.random.default_rng(n)
+    k, v = np.full((400, 2, 64), abs(size)), r.standard_normal((400, 2, 64))
+    for p in range(7):
+        v[p * PAGE:(p + 1) * PAGE] *= 2.0 ** (-p % 5)
+    k[63::128] *= 1 - 0.01 * np.sign(size)
+    check(pages_of(k, v), np.full((n, 4, 64), size), 400 - n, 0.125, 0, "f16", width=width)
