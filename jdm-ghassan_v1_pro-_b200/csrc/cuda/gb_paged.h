@@ -41,7 +41,7 @@ int gb_paged_append(const gb_paged* a, const void* qkv, long long ld_qkv, int H,
 int gb_paged_read(const gb_paged* a, void* k_out, long long ld_k, void* v_out, long long ld_v, cudaStream_t st);
 
 // out[row] = softmax(q K^T * scale) V for the H query heads of every new token over the tokens up to its own, which are in the pages; window > 0: over the last
-// `window` of them.  scale > 0, H a multiple of KV.  ws: gb_paged_attn_ws floats (0 or more; negative: why the arguments are refused), 16-byte aligned, this call's own until it
+// `window` of them.  Scores are fp32: what passes its range (3.4e38 after times log2 e) has no defined result.  scale > 0, H a multiple of KV.  ws: gb_paged_attn_ws floats (0 or more; negative: why the arguments are refused), 16-byte aligned, this call's own until it
 // is done.
 long long gb_paged_attn_ws(const gb_paged* a, int H, int window);
 int gb_paged_attn(const gb_paged* a, const void* q, long long ld_q, int H, float scale, int window, void* out, long long ld_o, float* ws,

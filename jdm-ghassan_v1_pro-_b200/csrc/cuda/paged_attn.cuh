@@ -26,7 +26,7 @@ __device__ __forceinline__ float pg_ex2(float x) {
   return r;
 }
 
-constexpr float PG_START = -1e30f;           // a running maximum before its first score
+constexpr float PG_START = -3.4028235e38f;   // a running maximum before its first score: no more than any
 // A maximum that a weight's exponent (offset + value scale - maximum, a few hundred) is not added to in one step: an fp32 number past 2^8 has steps of 2^-15 and more.
 __device__ __forceinline__ bool pg_far(float m) { return fabsf(m) > 256.f && m != PG_START; }
 

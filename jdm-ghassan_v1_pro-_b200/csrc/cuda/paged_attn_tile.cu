@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(256) paged_tile_join_kernel(const __grid_const
     const int rr = d.qt * L::ROWS + row, i = rr / G;
     if (rr >= s.n * G) continue;
     auto rec_of = [&](int x) { return records + (size_t)(x == c ? 2 * c + k : 2 * x) * L::REC; };
-    float top = -1e30f, sum = 0.f;
+    float top = PG_START, sum = 0.f;
     for (int x = c; x <= last; ++x) top = fmaxf(top, reinterpret_cast<const float2*>(rec_of(x) + L::ROWS * HD)[row].x);
     float4 acc[HD / 32];
 #pragma unroll

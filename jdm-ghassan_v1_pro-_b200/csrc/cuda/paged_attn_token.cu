@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(TK_THREADS, 1) paged_token_kernel(const __grid
       if (turn % TK_WARPS != warp) continue;
       const float2 at = *reinterpret_cast<const float2*>(my_rec + R * HD + 2 * r);
       const bool mine = my_item == c.item;
-      const float top = warp_max(mine ? at.x : -1e30f);
+      const float top = warp_max(mine ? at.x : PG_START);
       const float weight = !mine || at.y == 0.f ? 0.f : at.y * pg_ex2(at.x - top), sum = warp_sum(weight);
       const float f = sum == 0.f ? 0.f : __fdividef(1.f, sum);
 #pragma unroll
@@ -529,11 +529,11 @@ __global__ void __launch_bounds__(TJ_THREADS) paged_join_kernel(const __grid_con
   const float* parts = tk_parts(p, blocks);
   auto rec_of = [&](int j) { return parts + (size_t)(j == 0 ? 2 * c0 + k : 2 * (c0 + j)) * rec_n; };
   float2 ml[PG_MOST_BLOCKS / TJ_THREADS];
-  float top = -1e30f;
+  float top = PG_START;
 #pragma unroll
   for (int i = 0; i < PG_MOST_BLOCKS / TJ_THREADS; ++i) {
     const int j = i * TJ_THREADS + threadIdx.x;
-    ml[i] = j < n ? *reinterpret_cast<const float2*>(rec_of(j) + R * HD + 2 * r) : make_float2(-1e30f, 0.f);
+    ml[i] = j < n ? *reinterpret_cast<const float2*>(rec_of(j) + R * HD + 2 * r) : make_float2(PG_START, 0.f);
     top = fmaxf(top, ml[i].x);
   }
   top = warp_max(top);

@@ -132,3 +132,14 @@ def test_scores_that_leave_fp32_few_bits(n, size, width):
         v[p * PAGE:(p + 1) * PAGE] *= 2.0 ** (-p % 5)
     k[63::128] *= 1 - 0.01 * np.sign(size)
     check(pages_of(k, v), np.full((n, 4, 64), size), 400 - n, 0.125, 0, "f16", width=width)
+
+
+@pytest.mark.parametrize("n", [1, 5, 70])
+@pytest.mark.parametrize("start", [0, 300])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_scores_far_below_nothing(n, start, width):
+    """All scores are about -1e34: a finite soft-max all the same, the first token's over one key among them."""
+    r = np.random.default_rng(n)
+    k, v = np.full((start + n, 2, 64), -2.0 ** 43), r.standard_normal((start + n, 2, 64))
+    k[::3] *= 2
+    check(pages_of(k, v), np.full((n, 4, 64), 2.0 ** 66), start, 0.125, 0, "bf16", width=width)
