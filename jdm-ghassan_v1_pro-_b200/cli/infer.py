@@ -283,6 +283,7 @@ def main(argv: Optional[List[str]] = None) -> int:
         gen.engine.reset(1)
         gen.engine.prefill(torch.from_numpy(np.asarray(ids, dtype=np.int32)[None, :]).repeat(gen.engine.B, 1))
         lg = gen.engine.logits[0].float().cpu().numpy()
+        gen.check("logits")
         if a.out:
             lg.astype(np.float32).tofile(a.out)
         top = np.argsort(-lg)[:10]

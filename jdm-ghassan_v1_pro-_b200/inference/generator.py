@@ -47,6 +47,12 @@ class Generator:
             return self.tok.encode(prompt, add_bos=add_bos)
         return np.asarray(prompt, dtype=np.int32)
 
+    def check(self, what: str):
+        """Raises where the engine's pages were given what they do not hold (keys and values past its type, for one, which count as zero): every number since is
+        finite and wrong, and a record that nobody read would be told to a later call."""
+        if getattr(self.engine, "paged", False):
+            self.engine.check(what)
+
     def _cut_at_stop(self, toks: Sequence[int], stop_ids) -> "tuple[List[int], bool]":
         out = []
         for t in toks:
@@ -92,8 +98,7 @@ class Generator:
             toks, reasons = self._run_host(sp, ids, max_new, stop_ids, stop_strings, on_text)
         if not host_only:
             torch.cuda.synchronize()
-        if getattr(eng, "paged", False):                      # keys that 8 bits could not hold, for one
-            eng.check()
+        self.check("generation")
         t2 = time.perf_counter()
         res = GenerationResult(tokens=toks, prompt_tokens=n, prefill_seconds=t1 - t0, decode_seconds=t2 - t1,
                                stopped=reasons)
@@ -203,6 +208,7 @@ class Generator:
             lp = torch.log_softmax(eng.logits[0].double(), dim=-1)[ids[j + 1]]
             total -= float(lp)
             count += 1
+        self.check("scoring")
         return total, count
 
     def perplexity(self, ids: Sequence[int]) -> float:
@@ -242,6 +248,7 @@ class Generator:
         dec_ms = e1.elapsed_time(e2)
         n_timed = (new_tokens - 9) * eng.B
         toks = eng.transcript(new_tokens)
+        self.check("benchmark")
         return {"batch": eng.B, "prompt_len": prompt_len, "new_tokens": new_tokens, "decode_ms_per_token": dec_ms / (new_tokens - 9),
                 "decode_tokens_per_s": n_timed / (dec_ms / 1e3), "stored_weight_bytes": eng.weight_bytes,
                 "prefill_ms": e0.elapsed_time(e1_pre), "distinct_tokens": int(len(set(toks.reshape(-1).tolist())))}
