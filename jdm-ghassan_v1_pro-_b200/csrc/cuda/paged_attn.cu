@@ -21,9 +21,11 @@ int pg_sms() {
 
 using namespace gb;
 
+// New tokens of a sequence, at most: max_new may be more than there are rows.
+static long long gb_paged_most_new(const gb_paged* a) { return std::min<long long>(a->max_new, a->rows); }
 // Sequences of a launch: work is dealt by places counted in 32 bits, a sequence's being at most its pages or, for every 256 query rows, its pages and four more.
 static int gb_paged_most_seqs(const gb_paged* a, int H) {
-  const long long items = ((long long)a->max_new * (H / a->KV) + 255) / 256;
+  const long long items = (gb_paged_most_new(a) * (H / a->KV) + 255) / 256;
   const double places = (double)a->KV * items * (a->W + 4);
   return (int)std::min<double>(PG_MOST_SEQS, 2e9 / places);
 }
@@ -47,8 +49,8 @@ static PgAttn gb_paged_some(const PgAttn& p, int b0) {
 static int gb_paged_attn_args(const gb_paged* a, int H, int window) {
   if (const int rc = gb_paged_check(a)) return rc;
   if (H <= 0 || H % a->KV || window < 0 || H > 65535) return -1;
-  if ((long long)a->max_new * H > 0x7fffffffll) return -3;
-  if (a->max_new > 0 && gb_paged_most_seqs(a, H) < 1) return -3;
+  if (gb_paged_most_new(a) * H > 0x7fffffffll) return -3;
+  if (gb_paged_most_new(a) > 0 && gb_paged_most_seqs(a, H) < 1) return -3;
   return 0;
 }
 

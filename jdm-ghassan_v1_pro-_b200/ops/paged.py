@@ -207,8 +207,8 @@ def attn_scratch(B: int, width: int, kv_heads: int, head_dim: int, max_new: int,
     key = (B, width, kv_heads, head_dim, max_new, H, window, torch._C._cuda_getDevice())
     need = _scratch.get(key)
     if need is None:
-        # sizes alone count
-        a = _pack(4096, 4096, 4096, 4096, 1, kv_heads, head_dim, 4096, width, B, 4096, 0, 0, max_new, B * max_new, 0, 4096)
+        # sizes alone count, and rows do not: with fewer of them a launch takes more sequences, which need no less
+        a = _pack(4096, 4096, 4096, 4096, 1, kv_heads, head_dim, 4096, width, B, 4096, 0, 0, max_new, 1, 0, 4096)
         need = _protos().gb_paged_attn_ws(a, H, window)
         if need < 0:
             _lib.check_rc(int(need), "gb_paged_attn_ws")

@@ -175,6 +175,24 @@ def test_the_c_launchers_refuse_before_they_touch_the_device():
     assert three(ptr) == (0, 0, 0)
 
 
+@pytest.mark.skipif(not _lib.available(), reason="the kernel library is not built")
+def test_limits_go_by_the_rows_that_there_are(monkeypatch):
+    """max_new may be the most that tables hold: a call's own rows say how much there is to do."""
+    L = ctypes.CDLL(os.path.join(os.path.dirname(_lib.__file__), "..", "_gb200_cuda.so"))
+    L.gb_paged_attn_ws.argtypes, L.gb_paged_attn_ws.restype = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int], ctypes.c_longlong
+
+    def need(B, W, max_new, rows, KV=2, heads=4):
+        return L.gb_paged_attn_ws(P._pack(4096, 4096, 4096, 4096, 1, KV, 64, 4096, W, B, 4096, 4096, 4096, max_new, rows, 0, 4096), heads, 0)
+
+    monkeypatch.setattr(P, "_protos", lambda: L)
+    monkeypatch.setattr(P, "_scratch", {})
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    for B, W, max_new, rows in [(65535, 700, 44000, 100000), (3, 70000, 70000 * PAGE, 50), (1, 2 ** 24, 2 ** 30, 8), (1024, 32, 2048, 9000), (200, 32, 1, 200),
+                                (3, 8, 1, 3), (3, 8, 8, 11), (300, 2 ** 20, 5, 700)]:
+        assert P.attn_scratch(B, W, 2, 64, max_new, 4) >= need(B, W, max_new, rows) >= 0, (B, W, max_new, rows)
+    assert need(1, 2 ** 24, 2 ** 30, 2 ** 30) == -3           # this many rows are too many indeed
+
+
 def test_scales_are_the_smallest_powers_of_two():
     for x in [1e-30, 0.3, 1.0, 126.9, 127.0, np.nextafter(np.float32(127), np.float32(200)), 254.0, 6e4, 3e38]:
         s = float(scale_of(np.float32(x)))
