@@ -44,7 +44,7 @@ constexpr int PA_FEW = 64;
 // and not by conversions, a page's values are turned in registers, four tokens to a word, not stored byte by byte.  Six prompts of 7.7 thousand tokens (32/8 heads of 128,
 // 98 MB read, 40 written): 39 us, memory 43 % and issue slots 53 % busy.
 template <typename T, int HD, int ROPE, int NT>
-__global__ void __launch_bounds__(NT, NT == PA_FEW ? 8 : 1024 / NT) paged_append_kernel(const __grid_constant__ gb_paged a, const T* __restrict__ qkv, long long ld, int H,
+__global__ void __launch_bounds__(NT, NT == PA_FEW ? 8 : 1024 / NT) paged_append_kernel(const __grid_constant__ gb_paged a, int page0, const T* __restrict__ qkv, long long ld, int H,
                                                           T* __restrict__ q_out, long long ld_q, const float* __restrict__ qw,
                                                           const float* __restrict__ kw, float eps, const float* __restrict__ cs, int positions) {
   constexpr bool FEW = NT != 4 * HD;
@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(NT, NT == PA_FEW ? 8 : 1024 / NT) paged_append
   pdl_wait();
   const int b = blockIdx.z, g = blockIdx.x;
   const PgSeq s = pg_seq(a, b);
-  const int p = s.start / PG + (int)blockIdx.y;
+  const int p = s.start / PG + page0 + (int)blockIdx.y;
+  if ((unsigned)p >= (unsigned)a.W) return;
   const int lo = max(s.start, p * PG), hi = min(s.start + s.n, (p + 1) * PG);      // positions of this block
   if (lo >= hi) return;
   if (hi > positions) {
@@ -226,13 +227,14 @@ __global__ void __launch_bounds__(NT, NT == PA_FEW ? 8 : 1024 / NT) paged_append
 // byte, and neighbours fetch the rest of the sectors.
 constexpr int PR_THREADS = 128;
 template <typename T, int HD>
-__global__ void __launch_bounds__(PR_THREADS) paged_read_kernel(const __grid_constant__ gb_paged a, T* __restrict__ k_out, long long ld_k,
+__global__ void __launch_bounds__(PR_THREADS) paged_read_kernel(const __grid_constant__ gb_paged a, int page0, T* __restrict__ k_out, long long ld_k,
                                                                 T* __restrict__ v_out, long long ld_v) {
   constexpr int CH = HD / 16, NK = PG * CH / PR_THREADS, UD = HD / 8;
   pdl_wait();
   const int b = blockIdx.z, g = blockIdx.x;
   const PgSeq s = pg_seq(a, b);
-  const int p = s.start / PG + (int)blockIdx.y;
+  const int p = s.start / PG + page0 + (int)blockIdx.y;
+  if ((unsigned)p >= (unsigned)a.W) return;
   const int lo = max(s.start, p * PG), hi = min(s.start + s.n, (p + 1) * PG);
   if (lo >= hi) return;
   const int id = pg_page(a, b, p);
@@ -318,11 +320,28 @@ static bool gb_paged_rows_ok(const void* p, long long ld, long long width) {
     else { if (hd == 32) { CALL(__half, 32); } else if (hd == 64) { CALL(__half, 64); } else { CALL(__half, 128); } }     \
   } while (0)
 
-// Blocks along y: pages that max_new tokens can touch, wherever in a page they begin.
-static int gb_paged_grid(const gb_paged* a, dim3* grid) {
-  const int px = (int)std::min<long long>(((long long)a->max_new + 2 * GB_PAGE - 2) / GB_PAGE, a->W);
-  if (px > 65535 || a->B > 65535) return -3;
-  *grid = dim3(a->KV, px, a->B);
+// Launches over all pages that max_new tokens can touch, wherever in a page they begin, and all sequences: as many launches as it takes, since a grid has at most 65535 blocks along y
+// and z.  launch(part, b0, page0, grid): `part` has the sequences from b0 on, their pages count from page0.
+template <typename F>
+static int gb_paged_launches(const gb_paged* a, int grid_x, F&& launch) {
+  constexpr int MOST = 65535;
+  const int pages = (int)std::min<long long>(((long long)a->max_new + 2 * GB_PAGE - 2) / GB_PAGE, a->W);
+  for (int b0 = 0; b0 < a->B; b0 += MOST) {
+    gb_paged part = *a;
+    part.B = std::min(MOST, a->B - b0);
+    part.table += (long long)b0 * a->W;
+    part.start += b0;
+    if (a->count) {
+      part.first += b0;
+      part.count += b0;
+    } else {
+      part.rows = std::max(0ll, a->rows - b0);              // rows are counted from a launch's first sequence
+    }
+    for (int page0 = 0; page0 < pages; page0 += MOST) {
+      launch(part, a->count ? 0 : b0, page0, dim3(grid_x, std::min(MOST, pages - page0), part.B));
+      if (const int rc = gb_launch_rc()) return rc;
+    }
+  }
   return 0;
 }
 
@@ -332,24 +351,24 @@ extern "C" int gb_paged_append(const gb_paged* a, const void* qkv, long long ld_
   if (a->B == 0 || a->max_new == 0 || a->rows == 0) return 0;
   if (H <= 0 || H % a->KV || !cos_sin || (reinterpret_cast<uintptr_t>(cos_sin) & 15) || positions <= 0 || (rope_type != 0 && rope_type != 1)) return -1;
   if (!gb_paged_rows_ok(qkv, ld_qkv, (long long)(H + 2 * a->KV) * a->hd) || !gb_paged_rows_ok(q_out, ld_q, (long long)H * a->hd)) return -4;
-  dim3 grid;
-  if (const int rc = gb_paged_grid(a, &grid)) return rc;
-  grid.x += (H + 1) / 2;
   const bool few = a->max_new <= PA_FEW * 16 / a->hd;
-#define CALL(T, HD)                                                                                                                                                 \
-  do {                                                                                                                                                              \
-    if (few) GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, PA_FEW>), grid, dim3(PA_FEW), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
-    else GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, 4 * HD>), grid, dim3(4 * HD), st, *a, (const T*)qkv, ld_qkv, H, (T*)q_out, ld_q, qw, kw, eps, cos_sin, positions); \
+  return gb_paged_launches(a, a->KV + (H + 1) / 2, [&](const gb_paged& part, int row0, int page0, dim3 grid) {
+#define CALL(T, HD)                                                                                                                                                  \
+  do {                                                                                                                                                               \
+    const T* in = (const T*)qkv + row0 * ld_qkv;                                                                                                                     \
+    T* out = (T*)q_out + row0 * ld_q;                                                                                                                                \
+    if (few) GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, PA_FEW>), grid, dim3(PA_FEW), st, part, page0, in, ld_qkv, H, out, ld_q, qw, kw, eps, cos_sin, positions); \
+    else GB_PDL_LAUNCH((paged_append_kernel<T, HD, ROPE, 4 * HD>), grid, dim3(4 * HD), st, part, page0, in, ld_qkv, H, out, ld_q, qw, kw, eps, cos_sin, positions);  \
   } while (0)
-  if (rope_type == 0) {
-    constexpr int ROPE = 0;
-    GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
-  } else {
-    constexpr int ROPE = 1;
-    GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
-  }
+    if (rope_type == 0) {
+      constexpr int ROPE = 0;
+      GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
+    } else {
+      constexpr int ROPE = 1;
+      GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
+    }
 #undef CALL
-  return gb_launch_rc();
+  });
 }
 
 extern "C" int gb_paged_read(const gb_paged* a, void* k_out, long long ld_k, void* v_out, long long ld_v, cudaStream_t st) {
@@ -357,10 +376,9 @@ extern "C" int gb_paged_read(const gb_paged* a, void* k_out, long long ld_k, voi
   if (a->B == 0 || a->max_new == 0 || a->rows == 0) return 0;
   const long long width = (long long)a->KV * a->hd;
   if (!gb_paged_rows_ok(k_out, ld_k, width) || !gb_paged_rows_ok(v_out, ld_v, width)) return -4;
-  dim3 grid;
-  if (const int rc = gb_paged_grid(a, &grid)) return rc;
-#define CALL(T, HD) GB_PDL_LAUNCH((paged_read_kernel<T, HD>), grid, dim3(PR_THREADS), st, *a, (T*)k_out, ld_k, (T*)v_out, ld_v)
-  GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
+  return gb_paged_launches(a, a->KV, [&](const gb_paged& part, int row0, int page0, dim3 grid) {
+#define CALL(T, HD) GB_PDL_LAUNCH((paged_read_kernel<T, HD>), grid, dim3(PR_THREADS), st, part, page0, (T*)k_out + row0 * ld_k, ld_k, (T*)v_out + row0 * ld_v, ld_v)
+    GB_PAGED_TYPES(a->hd, a->is_bf16, CALL);
 #undef CALL
-  return gb_launch_rc();
+  });
 }

@@ -608,3 +608,59 @@ def test_nothing_to_do():
     P.attn(pool.p, q, empty, i32([]), 1, 4, 0.1, out=out)
     L.check_status()
     assert (out == 2).all() and k.shape == (0, 2, 64)
+
+
+# ---------------------------------------------------------------------------------------------- more than a grid has blocks along an axis
+@pytest.mark.parametrize("ragged", [False, True])
+def test_more_sequences_than_a_grid_has_rows(ragged):
+    """65535 blocks go along a grid's second and third axis; all three calls take what is more in several launches."""
+    P, L = ops()
+    B, hd = 65535 + 70, 32
+    g = torch.Generator("cuda").manual_seed(1)
+    pool = P.new_pages(B, 1, hd, "cuda")
+    table = torch.randperm(B, generator=g, device="cuda").to(torch.int32).view(B, 1)
+    count = torch.ones(B, dtype=torch.int32, device="cuda")
+    first = torch.arange(B, dtype=torch.int32, device="cuda")
+    if ragged:
+        count[5::3] = 0                                       # whose rows are nobody's
+        first = first.flip(0).contiguous()
+    kw = dict(first=first, count=count) if ragged else {}
+    start = torch.zeros(B, dtype=torch.int32, device="cuda")
+    qkv = torch.randn(B, 3 * hd, device="cuda", generator=g).half()
+    cs = torch.cat([torch.ones(1, hd // 2), torch.zeros(1, hd // 2)], 1).cuda()
+    out = [torch.full((B, hd), 9.0, dtype=torch.float16, device="cuda") for _ in range(4)]
+    P.append(pool, qkv, table, start, 1, cs, 1, q_out=out[0], **kw)
+    P.attn(pool, out[0], table, start, 1, 1, 0.2, out=out[1], **kw)
+    P.read(pool, table, start, 1, torch.float16, B, k_out=out[2], v_out=out[3], **kw)
+    L.check_status()
+    there = torch.zeros(B, dtype=torch.bool, device="cuda")
+    there[first[count > 0].long()] = True
+    assert all((x[~there] == 9).all() for x in out)
+    q, k, v = qkv.view(B, 3, hd).unbind(1)
+    assert torch.equal(out[0][there], q[there])
+    for got, want in ((out[2], k), (out[3], v)):              # half a step of a page that one token has, and float16's own
+        amax = want.float().abs().amax(1, keepdim=True)
+        assert ((got.float() - want.float()).abs() <= (1 / 127 + 2.0 ** -11) * amax)[there].all()
+    assert torch.equal(out[1][there], out[3][there])          # the soft-max over one key
+
+
+@pytest.mark.parametrize("n", [3, 100])
+def test_a_bound_of_more_pages_than_a_grid_has_rows(n):
+    """max_new may be far more than there is: as much as the table has places for."""
+    P, L = ops()
+    KV, hd, H, W = 2, 64, 4, 65535 + 40
+    pool = Pool(P, 4, KV, hd)
+    table = torch.full((1, W), -1, dtype=torch.int32, device="cuda")
+    table[0, :2] = i32([2, 0])
+    kw = dict(first=i32([0]), count=i32([n]))
+    qkv = torch.randn(n, (H + 2 * KV) * hd, device="cuda").half()
+    cs = cos_sin(n, hd)
+    q = P.append(pool.p, qkv, table, i32([0]), W * PAGE, cs, H, rope_type=1, **kw)
+    o = P.attn(pool.p, q, table, i32([0]), W * PAGE, H, 0.125, **kw)
+    k, v = P.read(pool.p, table, i32([0]), W * PAGE, torch.float16, n, **kw)
+    L.check_status()
+    s = Seq(KV, hd)
+    x = qkv.float().cpu().numpy().reshape(n, -1, hd)
+    s.append(rotate(x[:, H:H + KV], np.arange(n), cs.cpu().numpy(), 1), x[:, H + KV:])
+    check_attn(o, q, [s], [0], [n], [0], 0.125, 0, "f16", H, hd)
+    assert np.array_equal(v.double().cpu().numpy(), s.held()[1])
