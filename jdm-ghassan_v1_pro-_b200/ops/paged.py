@@ -163,6 +163,8 @@ def append(pages: Pages, qkv, table, start, max_new: int, cos_sin, H: int, *, fi
     if rope_type not in (0, 1):
         raise ValueError(f"paged append: rope_type is 0 or 1, not {rope_type}")
     a = _args(pages, pool, table, start, max_new, first, count, rows, dtype, "paged append")
+    if not (rows and max_new):
+        return q_out
     rc = _protos().gb_paged_append(a, qkv.data_ptr(), ld, H, q_out.data_ptr(), ld_q, None if qw is None else qw.data_ptr(),
                                    None if kw is None else kw.data_ptr(), eps, cos_sin.data_ptr(), cos_sin.shape[0], rope_type, _raw_stream(dev))
     if rc:
@@ -237,6 +239,8 @@ def read(pages: Pages, table, start, max_new: int, dtype, rows: int, *, first=No
         v_out, ld_v = _out(v_out, rows, KV * hd, None, dtype, dev, "paged read")
         at_v, v = v_out.data_ptr(), v_out.unflatten(1, (KV, hd))
     a = _args(pages, pool, table, start, max_new, first, count, rows, dtype, "paged read")
+    if not (rows and max_new):
+        return k, v
     rc = _protos().gb_paged_read(a, at_k, ld_k, at_v, ld_v, _raw_stream(dev))
     if rc:
         _lib.check_rc(rc, "gb_paged_read")

@@ -610,6 +610,22 @@ def test_nothing_to_do():
     assert (out == 2).all() and k.shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("B,W", [(0, 0), (2, 0), (0, 3)])
+def test_nothing_to_do_in_tables_of_no_pages(B, W):
+    """The same answer from all three calls."""
+    P, L = ops()
+    pool = Pool(P, 2, 2, 64).p
+    table = torch.empty(B, W, dtype=torch.int32, device="cuda")
+    kw = dict(first=i32([0] * B), count=i32([0] * B))
+    qkv, cs = torch.zeros(5, 8 * 64, dtype=torch.float16, device="cuda"), cos_sin(9, 64)
+    out = [torch.full((5, n), 2.0, dtype=torch.float16, device="cuda") for n in (256, 256, 128, 128)]
+    assert P.append(pool, qkv, table, i32([0] * B), 0, cs, 4, q_out=out[0], **kw) is out[0]
+    assert P.attn(pool, out[0], table, i32([0] * B), 0, 4, 0.1, out=out[1], **kw) is out[1]
+    k, v = P.read(pool, table, i32([0] * B), 0, torch.float16, 5, k_out=out[2], v_out=out[3], **kw)
+    L.check_status()
+    assert k.shape == v.shape == (5, 2, 64) and all((x == 2).all() for x in out)
+
+
 # ---------------------------------------------------------------------------------------------- more than a grid has blocks along an axis
 @pytest.mark.parametrize("ragged", [False, True])
 def test_more_sequences_than_a_grid_has_rows(ragged):
