@@ -34,8 +34,8 @@ __device__ __forceinline__ uint32_t pg_codes(const float* x, float inv) {
 }
 
 // Threads of a block with few new tokens a sequence, PA_FEW * 16 / HD at most: more such blocks are on an SM.  us of appending and reading back, these blocks against 4 HD threads:
-// 12/4 heads of 64, 1 and 16 tokens, one sequence 4.0 and 4.1 against 4.4 and 5.1, 512 of them 14.7 and 22.2 against 26.4 and 42.3; 32/8 heads of 128, 1 and 8 tokens, 256
-// sequences 24.4 and 34.0 against 64.1 and 88.2.
+// 12/4 heads of 64, 1 and 16 tokens, one sequence 4.1 and 4.2 against 4.5 and 5.2, 512 of them 14.8 and 22.3 against 26.7 and 42.3; 32/8 heads of 128, 1 and 8 tokens, 256
+// sequences 23.9 and 34.0 against 63.7 and 87.9.
 constexpr int PA_FEW = 64;
 
 // Blocks: (key head, behind them two query heads each; page of the new tokens; sequence): neighbours read neighbouring parts of the same rows.  HD / 16 lanes take a row:

@@ -5,8 +5,8 @@
 namespace gb {
 
 // Query rows a key head (tokens x heads of a group) up to which the token kernel runs: two columns of eight, which is all it has registers for.  The prompt kernel has 256
-// rows in hand, most of them empty here.  us, 12/4 heads of 64, 3 and 15 rows, token kernel against prompt kernel: one sequence of 2000 tokens 8.6
-// and 11.0 against 23.1 and 23.3, 32 of them 12.2 and 17.3 against 37.2 and 37.6, one of 30000 12.8 and 17.0 against 35.4 and 35.7; 16 rows, 32 of 2000, 8/2 heads: 14.5 against 25.4.
+// rows in hand, most of them empty here.  us, 12/4 heads of 64, 3 and 15 rows, token kernel against prompt kernel: one sequence of 2000 tokens 8.7
+// and 11.1 against 22.8 and 22.9, 32 of them 12.7 and 17.9 against 37.5 and 38.0, one of 30000 13.1 and 17.4 against 35.1 and 35.2; 16 rows, 32 of 2000, 8/2 heads: 14.9 against 24.8.
 constexpr int PG_TOKEN_ROWS = 16;
 constexpr int PG_MOST_BLOCKS = 256;          // blocks that pieces are dealt to, at most
 constexpr int PG_MOST_SEQS = 1024;           // sequences of one launch (their numbers are in shared memory); more are several launches

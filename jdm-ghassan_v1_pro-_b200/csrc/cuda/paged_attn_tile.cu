@@ -2,7 +2,7 @@
 //
 // Rows are (token, query head of the group) pairs of a key head, 256 of them an item, so any group size fills the tiles and a page is expanded once for all its query heads.
 // What bounds it: the exponentials (one a score, 16 a cycle and SM) and, at hd 128, the products about as much; neither is reached, since a warpgroup's step on a page is a chain of
-// scores, maxima, exponentials and products (2600 cycles, of which two warpgroups' exponentials are 1024).
+// scores, maxima, exponentials and products (2100 to 2200 cycles for both, of which the exponentials are 1024: special functions 49 % busy at hd 64, 47 % at hd 128).
 //
 // One block an SM: two warpgroups of soft-max threads, a row each; four warps expand the pages from codes in global memory to float16 integers in the swizzled layout of the MMAs
 // (integers up to 127 are exact, the scales go into the soft-max: a key scale into the score's factor, a value scale into the weight's exponent, as in paged_attn_token.cu, but that a
@@ -24,7 +24,7 @@ constexpr float TL_NONE = -1000.f;             // less than any exponent of a va
 template <int HD>
 struct Tl {
   // Tensor memory has 512 columns; a warpgroup (128 rows) takes HD of them for results and 64 for a buffer of the scores of a page, which its weights go over.  That leaves room for two
-  // buffers at hd 128 and three else, so that the products of a page run while the soft-max is at work on the next.  Measured beside it: one buffer of 128 keys, 7 ragged prompts
+  // buffers at hd 128 and three else, so that the products of a page run while the soft-max is at work on the next.  Measured beside it, with two places an item ahead of its pages (TlWalk): one buffer of 128 keys, 7 ragged prompts
   // (12/4 heads of 64) 188 us instead of 197, but 571 instead of 534 for 2048 tokens behind 14000 (32/8 heads of 128); four warpgroups with one buffer, scores
   // read twice for want of registers, 183, but 28.8 instead of 23.6 for a prompt of 1024.
   static constexpr int WGS = 2, BUFS = HD == 128 ? 2 : 3, ROWS = 128 * WGS, THREADS = 128 * (WGS + 2);

@@ -4,8 +4,8 @@
 // lengths are (mode "balanced"; the lengths are on the device and so is the dealing).  A warp streams its run through a ring of its own in shared memory, a bulk copy a
 // page of keys or values (4 KB at hd 64), and waits for nobody until its run is over: pieces of a (sequence, head) that lie in one warp are finished there, the others are joined
 // first in the block, then, across blocks, by a second kernel.  Where all items have a block each and few pages, a block takes an item and nothing is left to join (mode "item").
-// Whole calls: 192 sequences of 100 to 8000 tokens (8/2 heads of 64) 47.6 us, 4.2 TB/s of codes; one of 100001 (32/8 heads of 128) 44.2 us, 4.6 TB/s; 32 of 3 to 4095 (12/4 heads of
-// 64) 18.7 us, 1.9 TB/s, of which about 2.3 us pass before the first page is there and 3 us in joining a block's warps.
+// On the device: 192 sequences of 100 to 8000 tokens (8/2 heads of 64) 48.6 us, 4.1 TB/s of codes; one of 100001 (32/8 heads of 128) 44.1 us, 4.6 TB/s; 32 of 3 to 4095 (12/4 heads of
+// 64) 16.4 us, 2.1 TB/s, of which about 2.3 us pass before the first page is there and 3 us in joining a block's warps.
 //
 // A page is two products on the legacy tensor path, with the codes as float16 integers (exact): keys x queries and values x weights, so that
 // queries (8 columns) rather than keys are padded; 16 rows of queries would pad 3 of them to 16.  The order of the contracted dimensions is free as long as both operands have the
@@ -22,8 +22,8 @@ namespace gb {
 
 constexpr int TK_WARPS = 8, TK_THREADS = 32 * TK_WARPS;
 // Most pages a sequence may show in mode "item", which saves the second kernel and waits for a block's own pages only.  us, mode "item" against "balanced", 12/4 heads of 64, one
-// token behind 4, 8, 16, 24, 32 and 64 pages: one sequence 4.9, 5.4, 6.8, 8.3, 9.9, 16.1 against 7.0, 6.8, 8.2, 8.4, 8.6, 9.0; 32 sequences as long as each other gain more
-// (10.4 against 12.2 at 32 pages), but lengths are on the device and blocks of a ragged batch wait for the longest.
+// token behind 4, 8, 16, 24, 32 and 64 pages: one sequence 5.0, 5.5, 7.1, 8.8, 10.5, 17.0 against 7.1, 7.0, 8.3, 8.6, 8.6, 9.3; 32 sequences as long as each other gain more
+// (10.9 against 12.7 at 32 pages), but lengths are on the device and blocks of a ragged batch wait for the longest.
 constexpr int TK_ITEM_PAGES = 16;
 constexpr float TK_OFF = 15.f;               // the largest weight is held as 2^15 or (d is rounded up) a little less, the most float16 takes
 constexpr float TK_NONE = -1000.f;           // less than any exponent of a value scale

@@ -82,7 +82,7 @@ class InferenceEngine(TokenLoop):
         sequences on, the token step runs its projections and experts as tensor-core GEMMs over 16-bit copies of the
         weights (the ones the prompt pass keeps) instead of per-sequence GEMV kernels over the stored bytes; None
         takes ``GB200_DECODE_GEMM_MIN_BATCH`` (default 8), 0 turns it off.  ``kv_cache``: "16bit" or "q8" (8-bit pages; sequences end at
-        ``max_len``, and the kernel chain takes the token step)."""
+        ``max_len``; the kernel chain takes the token step, which for one sequence takes twice as long as the one kernel)."""
         cfg.validate()
         if kv_cache not in ("16bit", "q8"):
             raise ValueError("kv_cache is 16bit or q8, not %s" % kv_cache)
